@@ -101,6 +101,7 @@ def _asm_of(src, extra=()):
     key = (src, tuple(extra))
     if key not in _ASM_CACHE:
         _ASM_CACHE[key] = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only",
+                                          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",   # as build.FLAGS
                                           "-x", "hip", *extra, src, "-o", "-"], capture_output=True, text=True, check=True).stdout
     return _ASM_CACHE[key]
 
