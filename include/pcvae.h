@@ -421,6 +421,56 @@ int pcvae_bce_sigmoid(const float* x, const float* t, int64_t n, float* loss, fl
 int pcvae_relu_bwd(float* g, int64_t ldg, const float* y, int64_t ldy, int64_t rows, int cols, pcvae_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Layer norm over the rows of x [M, D] (1 <= D <= 16384), forward and backward.  No counterpart in the reference (its stacks are
+ * Linear + LeakyReLU only): for stacks with a norm between their layers.
+ *     fwd : mean[m], rstd[m] = 1 / sqrt(var + eps) (both optional, fp32) ;  y = (x - mean) rstd weight + bias (NULL: 1 / 0)
+ *           codes / scales: optionally the 8-bit form of x (below), from the same pass
+ *     bwd : h = (x - mean) rstd ;  dx = rstd (w g - mean(w g) - h mean(w g h)), times LeakyReLU'(x) with `leaky` (x is then a
+ *           LeakyReLU's output) ;  dweight[c] = sum_m g h,  dbias[c] = sum_m g (either may be NULL; accumulate: added to what is there).
+ *           The rows come as x OR as codes + scales (then x = NULL).  Sums are joined in a fixed order: the same bits every run.
+ *     x, y, g, dx: rows of `type` at any stride >= D (elements) and any alignment of their element; weight, bias, statistics, dweight
+ *     and dbias fp32.  dx may be g's own memory.  ws: pcvae_layer_norm_bwd_ws_bytes(M, D, type) bytes, contents irrelevant.
+ * ------------------------------------------------------------------------------------------- */
+#define PCVAE_ROW_F32 0
+#define PCVAE_ROW_BF16 1
+#define PCVAE_ROW_F16 2
+int pcvae_layer_norm_fwd(const void* x, int64_t ldx, int type, int64_t M, int D, const float* weight, const float* bias, float eps,
+                         void* y, int64_t ldy, float* mean, float* rstd, uint8_t* codes, int64_t ldc, uint8_t* scales, int64_t lds,
+                         pcvae_stream_t stream);
+size_t pcvae_layer_norm_bwd_ws_bytes(int64_t M, int D, int type);
+int pcvae_layer_norm_bwd(const void* g, int64_t ldg, int type, int64_t M, int D, const void* x, int64_t ldx, const uint8_t* codes,
+                         int64_t ldc, const uint8_t* scales, int64_t lds, const float* weight, const float* mean, const float* rstd,
+                         int leaky, void* dx, int64_t lddx, float* dweight, float* dbias, int accumulate, void* ws, size_t ws_bytes,
+                         pcvae_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Activation checkpoints in 8 bits: what a layer keeps of its input for the backward pass, at 1.03 bytes per value.  No counterpart in
+ * the reference (autograd keeps fp32).
+ *     Of every row, 32 consecutive columns share one scale byte s (2^(s - 127), s >= 10: the smallest power of two with
+ *     max |x| <= 448 * scale over the finite values, |x| held at 1.875 * 2^127); a code is the nearest OCP e4m3 multiple of it, ties to
+ *     even; a positive value never becomes zero (it becomes the smallest code: LeakyReLU' reads off the codes exactly); NaN and +-inf
+ *     become NaN.  codes [M, ldc], ldc a multiple of 16, >= 32 ceil(D / 32), 16-byte aligned, columns from D on hold code 0;
+ *     scales [M, ldsc], ldsc a multiple of 4, >= 4 ceil(D / 128), 4-byte aligned, bytes from ceil(D / 32) on unused.
+ *     pack       : x -> codes, scales                         unpack : codes, scales -> y (the values, rounded to `type`)
+ *     leaky_bwd  : g *= LeakyReLU'(x) in place, x the packed LeakyReLU output
+ *     bwd_weight : dW[N, K] = sum_m g[m, n] q[m, k],  db[n] = sum_m g[m, n] (NULL: not wanted), q [M, K] the packed values; accumulate:
+ *                  added to what is there.  With mean / rstd [M] (and weight / bias [K], NULL: 1 / 0) of a layer norm over q, q is
+ *                  replaced by (q - mean) rstd weight + bias.  fp32-exact products (bf16 components of g; the codes are exact in bf16),
+ *                  fp32 sums in a fixed order: the same bits every run.  ws: pcvae_act8_bwd_weight_ws_bytes(M, N, K) bytes.
+ * ------------------------------------------------------------------------------------------- */
+int pcvae_act8_pack(const void* x, int64_t ldx, int type, int64_t M, int64_t D, uint8_t* codes, int64_t ldc, uint8_t* scales,
+                    int64_t ldsc, pcvae_stream_t stream);
+int pcvae_act8_unpack(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t ldsc, int64_t M, int64_t D, void* y,
+                      int64_t ldy, int type, pcvae_stream_t stream);
+int pcvae_act8_leaky_bwd(void* g, int64_t ldg, int type, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t ldsc,
+                         int64_t M, int64_t D, pcvae_stream_t stream);
+size_t pcvae_act8_bwd_weight_ws_bytes(int64_t M, int64_t N, int64_t K);
+int pcvae_act8_bwd_weight(const void* g, int64_t ldg, int type, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t ldsc,
+                          int64_t M, int64_t N, int64_t K, const float* mean, const float* rstd, const float* weight,
+                          const float* bias, float* dW, int64_t lddw, float* db, int accumulate, void* ws, size_t ws_bytes,
+                          pcvae_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Offline metrics of generated slates                          analysis.py:5-30
  *   coverage_count : number of distinct item ids among ids[0..n) (ids outside [0, N) ignored); bits = scratch of
  *                    ceil(N / 32) words.  get_coverage = count / N.

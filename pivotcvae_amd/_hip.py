@@ -18,6 +18,9 @@ ACT_NONE, ACT_LEAKY, ACT_RELU = 0, 1, 2
 PREC_F32, PREC_BF16, PREC_BF16X3, PREC_SCREENED, PREC_BF16X6 = 0, 1, 2, 3, 4
 PREC_NAMES = {"f32": PREC_F32, "fp32": PREC_F32, "bf16": PREC_BF16, "bf16x3": PREC_BF16X3, "bf16x6": PREC_BF16X6}
 
+ROW_F32, ROW_BF16, ROW_F16 = 0, 1, 2
+ROW_TYPES = {torch.float32: ROW_F32, torch.bfloat16: ROW_BF16, torch.float16: ROW_F16}
+
 GEMM_FWD, GEMM_DX, GEMM_DX_ACC, GEMM_DW = 0, 1, 2, 3
 GEMM_X3 = 0x100   # OR-ed into a problem's kind: bf16x3 arithmetic (include/pcvae.h: PCVAE_GEMM_X3)
 GEMM_X6 = 0x200   # ... bf16x6 arithmetic: fp32-exact products on the bf16 matrix cores (PCVAE_GEMM_X6)
@@ -94,10 +97,19 @@ SIGNATURES = {
     "pcvae_normalize_rows_bwd": [_P, _L, _P, _P, _L, _P, _L, _L, _I, _P],
     "pcvae_bce_sigmoid": [_P, _P, _L, _P, _P, _F, _P],
     "pcvae_relu_bwd": [_P, _L, _P, _L, _L, _I, _P],
+    "pcvae_layer_norm_fwd": [_P, _L, _I, _L, _I, _P, _P, _F, _P, _L, _P, _P, _P, _L, _P, _L, _P],
+    "pcvae_layer_norm_bwd_ws_bytes": [_L, _I, _I],
+    "pcvae_layer_norm_bwd": [_P, _L, _I, _L, _I, _P, _L, _P, _L, _P, _L, _P, _P, _P, _I, _P, _L, _P, _P, _I, _P, _SZ, _P],
+    "pcvae_act8_pack": [_P, _L, _I, _L, _L, _P, _L, _P, _L, _P],
+    "pcvae_act8_unpack": [_P, _L, _P, _L, _L, _L, _P, _L, _I, _P],
+    "pcvae_act8_leaky_bwd": [_P, _L, _I, _P, _L, _P, _L, _L, _L, _P],
+    "pcvae_act8_bwd_weight_ws_bytes": [_L, _L, _L],
+    "pcvae_act8_bwd_weight": [_P, _L, _I, _P, _L, _P, _L, _L, _L, _L, _P, _P, _P, _P, _P, _L, _P, _I, _P, _SZ, _P],
     "pcvae_coverage_count": [_P, _L, _L, _P, _P, _P],
     "pcvae_ils": [_P, _L, _I, _P, _L, _I, _P, _P],
 }
-_RESTYPES = {"pcvae_last_error": _c.c_char_p, "pcvae_catalog_ws_bytes": _SZ, "pcvae_linear_group_ws_bytes": _SZ}
+_RESTYPES = {"pcvae_last_error": _c.c_char_p, "pcvae_catalog_ws_bytes": _SZ, "pcvae_linear_group_ws_bytes": _SZ,
+             "pcvae_layer_norm_bwd_ws_bytes": _SZ, "pcvae_act8_bwd_weight_ws_bytes": _SZ}
 
 _lib = None
 

@@ -12,8 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "lib", "libpcvae_hip.so")
 SOURCES = ["error.cpp", "elementwise.hip", "gemm_f32.hip", "catalog_f32.hip", "catalog_bf16.hip", "catalog_sparse.hip", "candidate_ce.hip", "catalog_sample.hip",
-           "catalog_api.cpp"]
-HEADERS = ["common.h", "catalog_plan.h", "catalog_x3.h", os.path.join("..", "..", "include", "pcvae.h")]
+           "layer_norm.hip", "act8.hip", "catalog_api.cpp"]
+HEADERS = ["common.h", "act8.h", "catalog_plan.h", "catalog_x3.h", os.path.join("..", "..", "include", "pcvae.h")]
 # -packed-fp32-ops: hipcc forms v_pk_add / mul / fma_f32 out of ordinary float code by itself, and some of their operand forms have been
 # seen to give wrong results on this chip; without the feature every one of them is two scalar instructions of the same rounding.
 # (The host pass does not know the feature and says so: harmless.)

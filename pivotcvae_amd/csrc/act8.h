@@ -1,0 +1,232 @@
+// Row operators in 32 bits over fp32 / bf16 / fp16 rows, and the 8-bit form of a row (layer_norm.hip, act8.hip).
+//
+// 8-bit rows: 32 consecutive columns share one power of two,
+//     scale = 2^(byte - 127),  byte = max(E - 8, 10),  E = biased exponent of max |x| (+ 1 where its significand exceeds 1.75),
+// so |x| / scale <= 448 and a value is its nearest OCP e4m3 multiple of the scale (ties to even).  A power of two costs e4m3 no
+// significand bit, makes the division exact - the rounding of the code is the only one - and keeps every value a bf16 as well: byte >= 10
+// keeps the smallest code (2^-9 scale) at 2^-126, a normal number.  Two additions serve the backward pass: a positive value never becomes
+// zero (it becomes the smallest code), so "x > 0" - LeakyReLU's derivative - reads off the code exactly; and NaN / +-inf become the NaN
+// code and stay out of the maximum, so one bad value does not hide its 31 neighbours.  |x| is held at 1.875 * 2^127 (the largest fp32 values
+// would round to 2^128).
+#pragma once
+#include "common.h"
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+
+namespace pcvae {
+
+constexpr int kAct8Block = 32;
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+// a 16-byte (8-byte, 4-byte) piece of memory at any alignment: rows of odd widths start anywhere.  One load / store instruction -
+// the global path takes unaligned accesses.
+template <int BYTES>
+struct __attribute__((packed)) Raw { uint32_t w[BYTES / 4]; };
+
+template <typename T> struct RowType;
+template <> struct RowType<float> {
+    static constexpr int VW = 4;
+    static __device__ __forceinline__ float one(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+    static __device__ __forceinline__ void widen(const Raw<16>& r, float (&v)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r.w[i]);
+    }
+    static __device__ __forceinline__ void narrow(const float (&v)[4], Raw<16>& r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = __float_as_uint(v[i]);
+    }
+};
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+
+template <> struct RowType<__bf16> {
+    static constexpr int VW = 8;
+    static __device__ __forceinline__ float one(const __bf16* p) {
+        return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16);
+    }
+    static __device__ __forceinline__ void put(__bf16* p, float v) { *p = (__bf16)v; }
+    static __device__ __forceinline__ void widen(const Raw<16>& r, float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(r.w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ void narrow(const float (&v)[8], Raw<16>& r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bf16x2_t h = __builtin_convertvector((f32x2_t{v[2 * i], v[2 * i + 1]}), bf16x2_t);
+            r.w[i] = __builtin_bit_cast(uint32_t, h);
+        }
+    }
+};
+template <> struct RowType<_Float16> {
+    static constexpr int VW = 8;
+    static __device__ __forceinline__ float one(const _Float16* p) { return (float)*p; }
+    static __device__ __forceinline__ void put(_Float16* p, float v) { *p = (_Float16)v; }
+    static __device__ __forceinline__ void widen(const Raw<16>& r, float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x2_t h = __builtin_bit_cast(f16x2_t, r.w[i]);
+            v[2 * i] = (float)h[0];
+            v[2 * i + 1] = (float)h[1];
+        }
+    }
+    static __device__ __forceinline__ void narrow(const float (&v)[8], Raw<16>& r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x2_t h = {(_Float16)v[2 * i], (_Float16)v[2 * i + 1]};
+            r.w[i] = __builtin_bit_cast(uint32_t, h);
+        }
+    }
+};
+
+// VW consecutive values of a row from column c on; columns from D on read 0 / are not written
+template <typename T>
+__device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&v)[RowType<T>::VW]) {
+    constexpr int VW = RowType<T>::VW;
+    if (c + VW <= D) {
+        RowType<T>::widen(*reinterpret_cast<const Raw<16>*>(row + c), v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] = c + i < D ? RowType<T>::one(row + c + i) : 0.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&v)[RowType<T>::VW]) {
+    constexpr int VW = RowType<T>::VW;
+    if (c + VW <= D) {
+        Raw<16> r;
+        RowType<T>::narrow(v, r);
+        *reinterpret_cast<Raw<16>*>(row + c) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < VW; ++i)
+            if (c + i < D) RowType<T>::put(row + c + i, v[i]);
+    }
+}
+
+// ---- reductions over 2^k neighbouring lanes, every lane gets the result ------------------------------------------------------------
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
+}
+template <int LANES, typename OP>
+__device__ __forceinline__ uint32_t lanes_reduce(uint32_t v, OP op) {
+    if constexpr (LANES >= 2) v = op(v, dpp<0xB1>(v));        // quad_perm 1,0,3,2
+    if constexpr (LANES >= 4) v = op(v, dpp<0x4E>(v));        // quad_perm 2,3,0,1
+    if constexpr (LANES >= 8) v = op(v, dpp<0x141>(v));       // row_half_mirror: the other quad of 8 (all lanes of a quad agree)
+    if constexpr (LANES >= 16) v = op(v, dpp<0x140>(v));      // row_mirror: the other half of 16
+    if constexpr (LANES >= 32) {
+        const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v = op(p[0], p[1]);
+    }
+    if constexpr (LANES >= 64) {
+        const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v = op(p[0], p[1]);
+    }
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return __uint_as_float(lanes_reduce<LANES>(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
+}
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    return lanes_reduce<LANES>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+}
+
+// ---- 8-bit blocks -----------------------------------------------------------------------------------------------------------------
+constexpr uint32_t kAct8Cap = 0x7f700000u;   // 1.875 * 2^127
+__device__ __forceinline__ uint32_t act8_magnitude(float x) {   // |x|'s bits as the block maximum counts them
+    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
+    return a >= 0x7f800000u ? 0u : (a < kAct8Cap ? a : kAct8Cap);
+}
+__device__ __forceinline__ uint32_t act8_byte(uint32_t top) {
+    const uint32_t e = (top + 0x1fffffu) >> 23;
+    return e > 18u ? e - 8u : 10u;
+}
+__device__ __forceinline__ float act8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float act8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// four values -> four codes (the lowest byte is the first)
+__device__ __forceinline__ uint32_t act8_codes(const float* x, float inv) {
+    float v[4];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float cap = __uint_as_float(kAct8Cap);
+        bad |= (__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u;
+        v[i] = fminf(fmaxf(x[i], -cap), cap) * inv;
+        v[i] = v[i] > 0.f ? fmaxf(v[i], 0x1p-9f) : v[i];
+    }
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r, true);
+    uint32_t codes = (uint32_t)r;
+    if (bad) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u) codes |= 0x7fu << (8 * i);
+    }
+    return codes;
+}
+// four codes -> their values
+__device__ __forceinline__ void act8_values(uint32_t codes, float scale, float* v) {
+    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    v[0] = a[0] * scale;
+    v[1] = a[1] * scale;
+    v[2] = b[0] * scale;
+    v[3] = b[1] * scale;
+}
+
+// a lane's VW values at columns [c, c + VW) of a block it shares with its 32 / VW - 1 neighbours -> codes and (first lane) the scale byte.
+// Every lane of the block takes part, whatever its columns (values from D on are zeros); columns from D on get code 0.
+template <int VW>
+__device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, uint8_t* codes, uint8_t* scales) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < VW; ++i) {
+        const uint32_t m = act8_magnitude(v[i]);
+        top = m > top ? m : top;
+    }
+    top = lanes_max<kAct8Block / VW>(top);
+    const uint32_t byte = act8_byte(top);
+    const float inv = act8_inverse(byte);
+    if (c < Dp) {
+        if constexpr (VW == 4) {
+            *reinterpret_cast<uint32_t*>(codes + c) = act8_codes(v, inv);
+        } else {
+            *reinterpret_cast<uint2*>(codes + c) = make_uint2(act8_codes(v, inv), act8_codes(v + 4, inv));
+        }
+        if ((c & (kAct8Block - 1)) == 0) scales[c / kAct8Block] = (uint8_t)byte;
+    }
+}
+// VW values of a row from its codes; 0 from Dp on (pad columns hold code 0)
+template <int VW>
+__device__ __forceinline__ void act8_load(const uint8_t* codes, const uint8_t* scales, int c, int Dp, float (&v)[VW]) {
+    if (c < Dp) {
+        const float s = act8_scale(scales[c / kAct8Block]);
+        if constexpr (VW == 4) {
+            act8_values(*reinterpret_cast<const uint32_t*>(codes + c), s, v);
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(codes + c);
+            act8_values(w.x, s, v);
+            act8_values(w.y, s, v + 4);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] = 0.f;
+    }
+}
+
+// host: the types of a row
+static inline int row_type_size(int t) { return t == PCVAE_ROW_F32 ? 4 : 2; }
+// codes [M, ldc >= ceil(D / 32) * 32] at a multiple of 16 bytes, scale bytes [M, lds >= ceil(D / 128) * 4] at a multiple of 4 (error.cpp)
+int act8_check(const char* who, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t M, int64_t D);
+static inline bool row_type_ok(int t) { return t == PCVAE_ROW_F32 || t == PCVAE_ROW_BF16 || t == PCVAE_ROW_F16; }
+
+}  // namespace pcvae

@@ -1,5 +1,6 @@
 // Host-side error text + ABI version for libpcvae_hip.so.
 #include "common.h"
+#include "act8.h"
 #include <atomic>
 #include <mutex>
 #include <cstdint>
@@ -135,3 +136,17 @@ extern "C" int pcvae_kernel_timer_read(float* ms, int* tags, int cap) {
 
 extern "C" int pcvae_abi_version(void) { return PCVAE_ABI_VERSION; }
 extern "C" const char* pcvae_last_error(void) { return pcvae::g_err; }
+
+namespace pcvae {
+int act8_check(const char* who, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t M, int64_t D) {
+    PCVAE_REQUIRE(M >= 0 && M <= (1LL << 40), "%s: rows in [0, 2^40] (got %lld)", who, (long long)M);
+    PCVAE_REQUIRE(D >= 1 && D <= (1 << 24), "%s: width in [1, 2^24] (got %lld)", who, (long long)D);
+    if (M == 0) return PCVAE_OK;
+    PCVAE_REQUIRE(codes && scales, "%s: null codes or scales", who);
+    PCVAE_REQUIRE(ldc >= cdiv(D, kAct8Block) * kAct8Block && ldc % 16 == 0 && (uintptr_t)codes % 16 == 0,
+                  "%s: codes need 16-byte aligned rows of at least %lld bytes", who, (long long)(cdiv(D, kAct8Block) * kAct8Block));
+    PCVAE_REQUIRE(lds >= cdiv(D, 4 * kAct8Block) * 4 && lds % 4 == 0 && (uintptr_t)scales % 4 == 0,
+                  "%s: scales need 4-byte aligned rows of at least %lld bytes", who, (long long)(cdiv(D, 4 * kAct8Block) * 4));
+    return PCVAE_OK;
+}
+}  // namespace pcvae

@@ -41,8 +41,13 @@ class BaseCVAE(nn.Module):
             if name in cls.__dict__:
                 setattr(cls, name, _in_mlp_arith(cls.__dict__[name]))
 
-    def __init__(self, embeddings, u_embeddings, slate_size, latent_size, no_user, device, fine_tune=False):
+    # (class attributes: modules pickled before these options existed have neither)
+    layer_norm = False             # a layer norm behind every hidden activation of the stacks (constructor argument)
+    activation_checkpoint = None   # what training keeps of the stacks' activations: fp32 (None) or 8 bits (set_activation_checkpoint)
+
+    def __init__(self, embeddings, u_embeddings, slate_size, latent_size, no_user, device, fine_tune=False, layer_norm=False):
         super().__init__()
+        self.layer_norm = bool(layer_norm)
         if fine_tune:
             raise NotImplementedError("fine_tune=True (trainable item/user tables) is outside the accelerated path: "
                                       "every reference model passes fine_tune=False (models/pivotcvae.py:319)")
@@ -87,6 +92,15 @@ class BaseCVAE(nn.Module):
         self.mlp_precision = name
         return self
 
+    def set_activation_checkpoint(self, name):
+        """what a train step keeps of the MLP stacks' activations for its backward pass: None (fp32, the default) or "e4m3" (8 bits: a
+        power-of-two scale per 32 columns, 1.03 bytes per value).  The forward pass and the loss are unchanged; weight gradients (and
+        the norms' gradients) are those at activations rounded to 2^-4 relative, LeakyReLU' stays exact"""
+        if name not in ops.ACTIVATION_CHECKPOINTS:
+            raise ValueError(f"activation checkpoint {name!r}: one of {ops.ACTIVATION_CHECKPOINTS}")
+        self.activation_checkpoint = name
+        return self
+
     @property
     def mlp_x3(self):   # the round-3 name of the switch (a module pickled before round 6 still carries it in its __dict__)
         d = self.__dict__
@@ -115,6 +129,22 @@ class BaseCVAE(nn.Module):
 
     def _mlp_layers(self, prefix, n):
         return [(getattr(self, f"{prefix}_{i + 1}").weight, getattr(self, f"{prefix}_{i + 1}").bias) for i in range(n)]
+
+    def _add_norms(self, prefix, struct, n):
+        """``layer_norm=True``: norms of the first n hidden activations of a stack, parameters ``<prefix>_norm_<i>.weight / .bias``"""
+        for i in range(n if self.layer_norm else 0):
+            if struct[i + 1] > ops.LAYER_NORM_MAX_WIDTH:
+                raise ValueError(f"layer norm over {struct[i + 1]} columns: at most {ops.LAYER_NORM_MAX_WIDTH}")
+            self.add_module(f"{prefix}_norm_{i + 1}", nn.LayerNorm(struct[i + 1]))
+
+    def _stack_options(self, prefix, n):
+        """ops.mlp / ops.mlp_heads arguments of a stack with n normed activations"""
+        if not self.layer_norm and self.activation_checkpoint is None:
+            return {}
+        norms = None
+        if self.layer_norm:
+            norms = [(m.weight, m.bias) for m in (getattr(self, f"{prefix}_norm_{i + 1}") for i in range(n))]
+        return dict(norms=norms, checkpoint=self.activation_checkpoint)
 
     def _head(self, name):
         m = getattr(self, name)

@@ -16,8 +16,8 @@ def _stack(module, prefix, struct):
 
 class UserListCVAEWithPrior(BaseCVAE):
     def __init__(self, embeddings, u_embeddings, slate_size, feature_size, latent_size, condition_size,
-                 encoder_struct, decoder_struct, prior_struct, no_user, device, fine_tune=False):
-        super().__init__(embeddings, u_embeddings, slate_size, latent_size, no_user, device, fine_tune)
+                 encoder_struct, decoder_struct, prior_struct, no_user, device, fine_tune=False, layer_norm=False):
+        super().__init__(embeddings, u_embeddings, slate_size, latent_size, no_user, device, fine_tune, layer_norm)
         self.feature_size = feature_size
         self.condition_size = condition_size
         self.encoderStruct = encoder_struct
@@ -35,19 +35,24 @@ class UserListCVAEWithPrior(BaseCVAE):
         self._n_prior = _stack(self, "prior", prior_struct)
         self.priorMu = nn.Linear(prior_struct[-1], latent_size)
         self.priorLogvar = nn.Linear(prior_struct[-1], latent_size)
+        self._add_norms("enc", encoder_struct, self._n_enc)
+        self._add_norms("dec", decoder_struct, self._n_dec - 1)
+        self._add_norms("prior", prior_struct, self._n_prior)
         self.to(self.device)
 
     def encode(self, emb, c, u_emb=None):
         x = ops.concat([emb, c] if self.noUser else [emb, c, u_emb])
-        return ops.mlp_heads(x, self._mlp_layers("enc", self._n_enc), self._head("encmu")[0], self._head("enclogvar")[0])
+        return ops.mlp_heads(x, self._mlp_layers("enc", self._n_enc), self._head("encmu")[0], self._head("enclogvar")[0],
+                             **self._stack_options("enc", self._n_enc))
 
     def decode(self, z, c, u_emb=None):
         x = ops.concat([z, c] if self.noUser else [z, c, u_emb])
-        return ops.mlp(x, self._mlp_layers("dec", self._n_dec), last_linear=True)
+        return ops.mlp(x, self._mlp_layers("dec", self._n_dec), last_linear=True, **self._stack_options("dec", self._n_dec - 1))
 
     def _prior_from(self, cond, u_emb):
         x = cond if self.noUser else ops.concat([cond, u_emb])
-        return ops.mlp_heads(x, self._mlp_layers("prior", self._n_prior), self._head("priorMu")[0], self._head("priorLogvar")[0])
+        return ops.mlp_heads(x, self._mlp_layers("prior", self._n_prior), self._head("priorMu")[0], self._head("priorLogvar")[0],
+                             **self._stack_options("prior", self._n_prior))
 
     def get_prior(self, r, u=None):
         return self._prior_from(self.get_condition(r), self._user_rows(u, r.shape[0]))

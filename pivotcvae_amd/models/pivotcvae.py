@@ -23,8 +23,8 @@ class UserPivotCVAE(BaseCVAE):
     INFER_RULE = "pi"
 
     def __init__(self, embeddings, u_embeddings, slate_size, feature_size, latent_size, condition_size,
-                 encoder_struct, psm_struct, scm_struct, prior_struct, no_user, device, fine_tune=False):
-        super().__init__(embeddings, u_embeddings, slate_size, latent_size, no_user, device, fine_tune)
+                 encoder_struct, psm_struct, scm_struct, prior_struct, no_user, device, fine_tune=False, layer_norm=False):
+        super().__init__(embeddings, u_embeddings, slate_size, latent_size, no_user, device, fine_tune, layer_norm)
         u = 0 if no_user else feature_size
         assert encoder_struct[0] == slate_size * feature_size + condition_size + u
         assert psm_struct[0] == latent_size + condition_size + u
@@ -46,6 +46,10 @@ class UserPivotCVAE(BaseCVAE):
         self._n_prior = _stack(self, "prior", prior_struct)
         self.priorMu = nn.Linear(prior_struct[-1], latent_size)
         self.priorLogvar = nn.Linear(prior_struct[-1], latent_size)
+        self._add_norms("enc", encoder_struct, self._n_enc)
+        self._add_norms("psm", psm_struct, self._n_psm - 1)
+        self._add_norms("scm", scm_struct, self._n_scm - 1)
+        self._add_norms("prior", prior_struct, self._n_prior)
         self.pivot_override = None  # test hook: feed recorded Categorical draws back in
         self.last_pivot = None      # pivot item ids chosen by the most recent decode()
         self.to(self.device)
@@ -59,16 +63,19 @@ class UserPivotCVAE(BaseCVAE):
     def params_without_grad(self):
         """trainable parameters that never receive a gradient under ANY pivot rule: the PSM stack (its output is
         either ignored or feeds a non-differentiable argmax / sample).  torch.optim.Adam skips them (grad is None)."""
-        return [p for i in range(self._n_psm) for p in getattr(self, f"psm_{i + 1}").parameters()]
+        names = [f"psm_{i + 1}" for i in range(self._n_psm)] + [f"psm_norm_{i + 1}" for i in range(self._n_psm - 1) if self.layer_norm]
+        return [p for name in names for p in getattr(self, name).parameters()]
 
     # ---- encoder / prior -----------------------------------------------------------------------
     def encode(self, emb, c, u_emb=None):
         x = ops.concat([emb, c] if self.noUser else [emb, c, u_emb])
-        return ops.mlp_heads(x, self._mlp_layers("enc", self._n_enc), self._head("encmu")[0], self._head("enclogvar")[0])
+        return ops.mlp_heads(x, self._mlp_layers("enc", self._n_enc), self._head("encmu")[0], self._head("enclogvar")[0],
+                             **self._stack_options("enc", self._n_enc))
 
     def _prior_from(self, cond, u_emb):
         x = cond if self.noUser else ops.concat([cond, u_emb])
-        return ops.mlp_heads(x, self._mlp_layers("prior", self._n_prior), self._head("priorMu")[0], self._head("priorLogvar")[0])
+        return ops.mlp_heads(x, self._mlp_layers("prior", self._n_prior), self._head("priorMu")[0], self._head("priorLogvar")[0],
+                             **self._stack_options("prior", self._n_prior))
 
     def get_prior(self, r, u=None):
         return self._prior_from(self.get_condition(r), self._user_rows(u, r.shape[0]))
@@ -106,14 +113,14 @@ class UserPivotCVAE(BaseCVAE):
     def decode(self, z, c, u_emb=None, true_pivot=[], sample_offset=None, pivot_row=None):
         B = z.shape[0]
         x = ops.concat([z, c] if self.noUser else [z, c, u_emb])
-        pivot_output = ops.mlp(x, self._mlp_layers("psm", self._n_psm), last_linear=True)
+        pivot_output = ops.mlp(x, self._mlp_layers("psm", self._n_psm), last_linear=True, **self._stack_options("psm", self._n_psm - 1))
         pivot_emb = self.pick_pivot(pivot_output, true_pivot, sample_offset, pivot_row)
         return self._complete(z, c, u_emb, pivot_emb)
 
     def _complete(self, z, c, u_emb, pivot_emb):
         B = z.shape[0]
         x = ops.concat([z, c, pivot_emb] if self.noUser else [z, c, pivot_emb, u_emb])
-        rest = ops.mlp(x, self._mlp_layers("scm", self._n_scm), last_linear=True)
+        rest = ops.mlp(x, self._mlp_layers("scm", self._n_scm), last_linear=True, **self._stack_options("scm", self._n_scm - 1))
         return ops.concat([pivot_emb, rest]).reshape(B, self.slate_size, self.feature_size)
 
     # ---- reference entry points -----------------------------------------------------------------
@@ -151,7 +158,8 @@ class UserPivotCVAE(BaseCVAE):
         the reference either.
         """
         B, S = s.shape
-        if self.TRAIN_RULE == "gt" and self.FUSED_TRAIN_PATH and r.shape[1] == S and \
+        plain = not self.layer_norm and self.activation_checkpoint is None   # the fused launches know neither option
+        if plain and self.TRAIN_RULE == "gt" and self.FUSED_TRAIN_PATH and r.shape[1] == S and \
                 ops.heads_adjacent(self.encmu, self.enclogvar) and ops.heads_adjacent(self.priorMu, self.priorLogvar):
             return self._loss_fused(s, r, u, beta, n_neg, eps, keep_mask, mask_seed, row_offset, inv_count, eps_offset, terms_only,
                                     candidates, n_items)

@@ -11,7 +11,7 @@ import torch
 
 from . import _hip
 from ._hip import (ACT_LEAKY, ACT_NONE, ACT_RELU, GEMM_DW, GEMM_DX, GEMM_DX_ACC, GEMM_FWD, GEMM_GROUP_MAX, GEMM_X3, GEMM_X6, PREC_BF16, PREC_BF16X3, PREC_BF16X6,
-                   PREC_F32, PREC_SCREENED, GemmDesc, check, lib, ptr, require_device, stream)
+                   PREC_F32, PREC_SCREENED, ROW_TYPES, GemmDesc, check, lib, ptr, require_device, stream)
 
 F32 = torch.float32
 
@@ -468,13 +468,447 @@ class _MLPHeads(torch.autograd.Function):
         return (g, None) + tuple(grads)
 
 
-def mlp_heads(x, trunk, head_a, head_b):
+def mlp_heads(x, trunk, head_a, head_b, norms=None, checkpoint=None, norm_eps=1e-5):
     """trunk: list of (weight, bias) with LeakyReLU after every layer; head_a / head_b: (weight, bias), linear.
-    -> (head_a(trunk(x)), head_b(trunk(x)))"""
+    -> (head_a(trunk(x)), head_b(trunk(x))).  norms: one (weight, bias) per trunk layer - a layer norm behind its activation;
+    checkpoint = "e4m3": what the backward pass reads of the activations is kept in 8 bits (_KeptStack)"""
+    if norms is not None or checkpoint is not None:
+        return _kept_stack(x, trunk, [head_a, head_b], False, norms, checkpoint, norm_eps)
     flat = []
     for W, b in list(trunk) + [head_a, head_b]:
         flat += [W, b]
     return _MLPHeads.apply(x, len(trunk), *flat)
+
+
+# --------------------------------------------------------------- layer norm, activation checkpoints in 8 bits (csrc/layer_norm.hip, act8.hip)
+ACT8_BLOCK = 32
+ACTIVATION_CHECKPOINTS = (None, "e4m3")
+LAYER_NORM_MAX_WIDTH = 16384
+
+
+def _one_device(*tensors):
+    """every tensor on the same ROCm device -> that device"""
+    require_device(*tensors)
+    devs = {t.device for t in tensors if t is not None}
+    if len(devs) != 1:
+        raise RuntimeError(f"tensors on different devices: {sorted(str(d) for d in devs)}")
+    return devs.pop()
+
+
+class _device_guard:
+    """launches inside go to `dev`'s current stream, whatever device is current outside"""
+
+    def __init__(self, dev):
+        self.dev = dev
+
+    def __enter__(self):
+        self.prev = None
+        if self.dev.index is not None and self.dev.index != torch.cuda.current_device():
+            self.prev = torch.cuda.current_device()
+            torch.cuda.set_device(self.dev.index)
+
+    def __exit__(self, *exc):
+        if self.prev is not None:
+            torch.cuda.set_device(self.prev)
+        return False
+
+
+def _row_type(t):
+    if t.dtype not in ROW_TYPES:
+        raise TypeError(f"expected float32, bfloat16 or float16, got {t.dtype}")
+    return ROW_TYPES[t.dtype]
+
+
+def _rows(t):
+    """[..., D] as a 2-D view with contiguous, non-overlapping rows (copied only if the layout forces it)"""
+    if t.dim() < 1:
+        raise ValueError("expected [..., D], got a scalar")
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.numel() else t.reshape(t.shape[:-1].numel(), t.shape[-1])
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _vector(t, n, what):
+    """an fp32 [n] parameter / statistic (None passes)"""
+    if t is None:
+        return None
+    if t.dtype != F32:
+        raise TypeError(f"{what}: expected float32, got {t.dtype}")
+    if tuple(t.shape) != (n,):
+        raise RuntimeError(f"{what}: expected shape ({n},), got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _check_checkpoint(name):
+    if name not in ACTIVATION_CHECKPOINTS:
+        raise ValueError(f"activation checkpoint {name!r}: one of {ACTIVATION_CHECKPOINTS}")
+    return name
+
+
+class Act8:
+    """Rows kept in 8 bits: e4m3 codes, one power-of-two scale per 32 columns of a row (include/pcvae.h).  `shape` is that of the
+    tensor that was packed, `dtype` its type; rows are its leading dimensions flattened."""
+
+    __slots__ = ("codes", "scales", "shape", "dtype")
+
+    def __init__(self, codes, scales, shape, dtype=F32):
+        M, D = torch.Size(shape[:-1]).numel(), shape[-1]
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise TypeError("Act8: codes and scales are uint8")
+        if D < 1:
+            raise ValueError("Act8: width 0")
+        if tuple(codes.shape) != (M, self.code_width(D)) or tuple(scales.shape) != (M, self.scale_width(D)):
+            raise RuntimeError(f"Act8: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} do not hold {tuple(shape)}")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise ValueError("Act8: codes and scales are contiguous")
+        self.codes, self.scales, self.shape, self.dtype = codes, scales, torch.Size(shape), dtype
+
+    @staticmethod
+    def code_width(D):
+        return -(-D // ACT8_BLOCK) * ACT8_BLOCK
+
+    @staticmethod
+    def scale_width(D):
+        return -(-D // (4 * ACT8_BLOCK)) * 4
+
+    @classmethod
+    def empty(cls, shape, dtype, device):
+        M, D = torch.Size(shape[:-1]).numel(), shape[-1]
+        return cls(torch.empty(M, cls.code_width(D), dtype=torch.uint8, device=device),
+                   torch.empty(M, cls.scale_width(D), dtype=torch.uint8, device=device), shape, dtype)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.scales.numel()
+
+    def _args(self):   # the four arguments of the C ABI
+        return ptr(self.codes), self.codes.shape[1], ptr(self.scales), self.scales.shape[1]
+
+    def unpack(self, dtype=None):
+        """the values the codes stand for (rounded to `dtype`; default: the type that was packed)"""
+        dtype = dtype or self.dtype
+        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        t, M, D = _row_type(out), self.codes.shape[0], self.shape[-1]
+        _one_device(self.codes, self.scales)
+        with _device_guard(self.device):
+            check(lib().pcvae_act8_unpack(*self._args(), M, D, ptr(out), D, t, stream()), "act8_unpack")
+        return out
+
+
+def act8_pack(x):
+    """x [..., D] (fp32 / bf16 / fp16) -> Act8: 1.03 bytes per value; relative error at most 2^-4 per value above 2^-14 of its block's
+    largest, the sign of "x > 0" exact"""
+    dev = _one_device(x)
+    t, rows = _row_type(x), _rows(x)
+    ck = Act8.empty(x.shape, x.dtype, dev)
+    with _device_guard(dev):
+        check(lib().pcvae_act8_pack(ptr(rows), _ld(rows), t, rows.shape[0], rows.shape[1], *ck._args(), stream()), "act8_pack")
+    return ck
+
+
+def act8_leaky_bwd_(g, ck):
+    """g *= LeakyReLU'(x) in place, x the LeakyReLU output that `ck` holds"""
+    dev = _one_device(g, ck.codes, ck.scales)
+    if g.shape != ck.shape:
+        raise RuntimeError(f"act8_leaky_bwd: gradient {tuple(g.shape)} of activations {tuple(ck.shape)}")
+    rows = _rows(g)
+    if rows.data_ptr() != g.data_ptr():
+        raise ValueError("act8_leaky_bwd: works in place on rows with unit column stride")
+    with _device_guard(dev):
+        check(lib().pcvae_act8_leaky_bwd(ptr(rows), _ld(rows), _row_type(g), *ck._args(), rows.shape[0], rows.shape[1], stream()),
+              "act8_leaky_bwd")
+    return g
+
+
+def act8_bwd_weight_raw(gy, ck, dW=None, db=None, norm=None):
+    """the weight gradient of a linear layer whose input was kept in 8 bits: dW[N, K] = gy^T q, db[N] = column sums of gy
+    (gy [..., N] fp32 / bf16 / fp16, products and sums fp32) -> (dW, db).  Given buffers are accumulated into; None: new ones.
+    norm = (mean, rstd, weight, bias): the layer's input was layer_norm(q) with those statistics (weight / bias may be None)."""
+    mean, rstd, w, b = norm if norm is not None else (None,) * 4
+    dev = _one_device(gy, ck.codes, ck.scales, dW, db, mean, rstd, w, b)
+    t, rows = _row_type(gy), _rows(gy)
+    M, N, K = rows.shape[0], rows.shape[1], ck.shape[-1]
+    if M != ck.codes.shape[0]:
+        raise RuntimeError(f"act8_bwd_weight: {M} gradient rows for {ck.codes.shape[0]} kept rows")
+    if norm is not None:
+        mean, rstd = _vector(mean, M, "act8_bwd_weight: mean"), _vector(rstd, M, "act8_bwd_weight: rstd")
+        if mean is None or rstd is None:
+            raise ValueError("act8_bwd_weight: norm needs its mean and rstd")
+        w, b = _vector(w, K, "act8_bwd_weight: norm weight"), _vector(b, K, "act8_bwd_weight: norm bias")
+    if (dW is None) != (db is None):
+        raise ValueError("act8_bwd_weight: dW and db are accumulated into together")
+    accumulate = dW is not None
+    if accumulate:
+        if dW.dtype != F32 or db.dtype != F32:
+            raise TypeError("act8_bwd_weight: dW and db are float32")
+        if tuple(dW.shape) != (N, K) or tuple(db.shape) != (N,) or not db.is_contiguous() or (K > 1 and dW.stride(1) != 1) or \
+                (N > 1 and dW.stride(0) < K):
+            raise RuntimeError(f"act8_bwd_weight: dW ({N}, {K}) with contiguous rows and contiguous db ({N},) expected, got "
+                               f"{tuple(dW.shape)} / {tuple(db.shape)}")
+    else:
+        dW, db = torch.empty(N, K, dtype=F32, device=dev), torch.empty(N, dtype=F32, device=dev)
+    with _device_guard(dev):
+        nbytes = lib().pcvae_act8_bwd_weight_ws_bytes(M, N, K)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        check(lib().pcvae_act8_bwd_weight(ptr(rows), _ld(rows), t, *ck._args(), M, N, K, ptr(mean), ptr(rstd), ptr(w), ptr(b), ptr(dW),
+                                          _ld(dW), ptr(db), int(accumulate), ptr(ws), nbytes, stream()), "act8_bwd_weight")
+    return dW, db
+
+
+def layer_norm_fwd_raw(x, weight=None, bias=None, eps=1e-5, checkpoint=None):
+    """layer norm over the last dimension of x [..., D] (fp32 / bf16 / fp16, D <= 16384; weight / bias [D] fp32 or None)
+    -> (y, mean, rstd, kept): y like x, fp32 statistics per row, kept = x in 8 bits (checkpoint = "e4m3", same pass) or None"""
+    _check_checkpoint(checkpoint)
+    dev = _one_device(x, weight, bias)
+    t, rows = _row_type(x), _rows(x)
+    M, D = rows.shape
+    weight, bias = _vector(weight, D, "layer_norm: weight"), _vector(bias, D, "layer_norm: bias")
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    mean, rstd = torch.empty(M, dtype=F32, device=dev), torch.empty(M, dtype=F32, device=dev)
+    ck = Act8.empty(x.shape, x.dtype, dev) if checkpoint else None
+    with _device_guard(dev):
+        check(lib().pcvae_layer_norm_fwd(ptr(rows), _ld(rows), t, M, D, ptr(weight), ptr(bias), float(eps), ptr(y), D, ptr(mean),
+                                         ptr(rstd), *(ck._args() if ck else (None, 0, None, 0)), stream()), "layer_norm_fwd")
+    return y, mean, rstd, ck
+
+
+def layer_norm_bwd_raw(gy, x, weight, mean, rstd, dweight=None, dbias=None, leaky=False):
+    """-> (dx, dweight, dbias) of layer_norm at x (a tensor of gy's type, or the Act8 the forward kept).  leaky: x is a LeakyReLU's
+    output and dx is taken through it, to its input.  Given dweight / dbias buffers are accumulated into; None: new ones."""
+    kept = isinstance(x, Act8)
+    parts = (x.codes, x.scales) if kept else (x,)
+    dev = _one_device(gy, *parts, weight, mean, rstd, dweight, dbias)
+    if gy.shape != x.shape:
+        raise RuntimeError(f"layer_norm: gradient {tuple(gy.shape)} of rows {tuple(x.shape)}")
+    if not kept and gy.dtype != x.dtype:
+        raise TypeError(f"layer_norm: gradient of type {gy.dtype} at rows of type {x.dtype}")
+    t, g = _row_type(gy), _rows(gy)
+    M, D = g.shape
+    weight = _vector(weight, D, "layer_norm: weight")
+    mean, rstd = _vector(mean, M, "layer_norm: mean"), _vector(rstd, M, "layer_norm: rstd")
+    if mean is None or rstd is None:
+        raise ValueError("layer_norm: the backward needs mean and rstd of the forward")
+    if (dweight is None) != (dbias is None):
+        raise ValueError("layer_norm: dweight and dbias are accumulated into together")
+    accumulate = dweight is not None
+    if accumulate:
+        for b in (dweight, dbias):
+            _vector(b, D, "layer_norm: gradient buffer")
+            if not b.is_contiguous():
+                raise ValueError("layer_norm: gradient buffers are contiguous")
+    else:
+        dweight, dbias = torch.empty(D, dtype=F32, device=dev), torch.empty(D, dtype=F32, device=dev)
+    rows = None if kept else _rows(x)
+    dx = torch.empty(gy.shape, dtype=gy.dtype, device=dev)
+    with _device_guard(dev):
+        nbytes = lib().pcvae_layer_norm_bwd_ws_bytes(M, D, t)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        check(lib().pcvae_layer_norm_bwd(ptr(g), _ld(g), t, M, D, ptr(rows), 0 if kept else _ld(rows),
+                                         *(x._args() if kept else (None, 0, None, 0)), ptr(weight), ptr(mean), ptr(rstd), int(bool(leaky)),
+                                         ptr(dx), D, ptr(dweight), ptr(dbias), int(accumulate), ptr(ws), nbytes, stream()),
+              "layer_norm_bwd")
+    return dx, dweight, dbias
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint):
+        y, mean, rstd, ck = layer_norm_fwd_raw(x, weight, bias, eps, checkpoint)
+        ctx.kept = ck.shape if ck else None
+        ctx.save_for_backward(weight, mean, rstd, *((ck.codes, ck.scales) if ck else (x,)))
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        weight, mean, rstd, *rest = ctx.saved_tensors
+        x = Act8(rest[0], rest[1], ctx.kept, gy.dtype) if ctx.kept is not None else rest[0]
+        dx, dw, db = layer_norm_bwd_raw(gy, x, weight, mean, rstd)
+        need = ctx.needs_input_grad
+        return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=None):
+    """layer norm over the last dimension (layer_norm_fwd_raw), differentiable; checkpoint = "e4m3": the backward pass reads x from its
+    8-bit form (1.03 bytes per value kept) instead of x itself"""
+    return _LayerNorm.apply(x, weight, bias, float(eps), _check_checkpoint(checkpoint))
+
+
+class _KeptStack(torch.autograd.Function):
+    """_MLP / _MLPHeads with a layer norm behind every hidden activation and / or with the layers' inputs kept in 8 bits.
+
+    layer i: z = W h + b, a = LeakyReLU(z) (the top layer of a headless stack: a = z if last_linear); a hidden a is the next layer's
+    input, through its norm if there are norms.  Kept for the backward pass: the input x and the hidden a (8 bits with a checkpoint;
+    fp32 otherwise, and then the norms' outputs too) and the norms' statistics.  One kept a serves the three places of the backward
+    pass that read it: the next layer's weight gradient (act8_bwd_weight, the norm folded in), the norm's own backward, LeakyReLU'."""
+
+    @staticmethod
+    def forward(ctx, x, spec, *params):
+        ctx.x3 = _MLP_MODE
+        n, heads, last_linear, normed, checkpoint, eps, train = spec
+        require_device(x, *params)
+        x = _c2d(x)
+        layers = [params[2 * i:2 * i + 2] for i in range(n + heads)]
+        hidden = n if heads or not last_linear else n - 1        # activated layers
+        inner = n if heads else n - 1                            # ... whose output another layer reads
+        norms = [params[2 * (n + heads) + 2 * i:2 * (n + heads) + 2 * i + 2] for i in range(inner if normed else 0)]
+        keep, stats = [], []   # keep[i] = (what layer i's weight gradient reads, what its input's activation left); stats[i]: norm i's
+
+        def kept(t):
+            return act8_pack(t) if checkpoint and train else t
+
+        h = x
+        with gemm_span():
+            keep.append((kept(x), None))
+            for i in range(n):
+                W, b = layers[i]
+                a = linear_fwd_raw(h, W, b, ACT_LEAKY if i < hidden else ACT_NONE)
+                h = a
+                if i < inner:
+                    if normed:
+                        h, mean, rstd, ck = layer_norm_fwd_raw(a, norms[i][0], norms[i][1], eps, checkpoint if train else None)
+                        stats.append((mean, rstd))
+                        keep.append((ck, ck) if ck is not None else (h, a))
+                    else:
+                        k = kept(a)
+                        keep.append((k, k))
+            outs = [linear_fwd_raw(h, *layers[n + j], ACT_NONE) for j in range(heads)] or [h]
+        ctx.spec, ctx.hidden, ctx.inner = spec, hidden, inner
+        if train:
+            ctx.direct = [p.grad if (p.is_leaf and p.requires_grad and p.grad is not None and p.grad.is_cuda
+                                     and p.grad.shape == p.shape and p.grad.is_contiguous()) else None for p in params]
+            flat, ctx.layout = [], []
+            for pair in keep:
+                place = []
+                for k, t in enumerate(pair):
+                    if t is None:
+                        place.append(None)
+                    elif k == 1 and t is pair[0]:
+                        place.append("same")
+                    elif isinstance(t, Act8):
+                        place.append((len(flat), t.shape))
+                        flat += [t.codes, t.scales]
+                    else:
+                        place.append((len(flat), None))
+                        flat.append(t)
+                ctx.layout.append(place)
+            ctx.n_flat = len(flat)
+            top = [outs[0]] if not heads and not last_linear else []   # its LeakyReLU' needs the activated output itself
+            ctx.save_for_backward(*flat, *[t for st in stats for t in st], *top, *params)
+        return tuple(outs) if heads else outs[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *gs):
+        with gemm_span(), mlp_arith(ctx.x3):
+            return _KeptStack._backward_impl(ctx, *gs)
+
+    @staticmethod
+    def _backward_impl(ctx, *gs):
+        n, heads, last_linear, normed, checkpoint, eps, _ = ctx.spec
+        inner = ctx.inner
+        saved = list(ctx.saved_tensors)
+        keep = []
+        for place in ctx.layout:
+            got = []
+            for p in place:
+                if p is None or p == "same":
+                    got.append(got[0] if p == "same" else None)
+                else:
+                    got.append(saved[p[0]] if p[1] is None else Act8(saved[p[0]], saved[p[0] + 1], p[1]))
+            keep.append(got)
+        pos = ctx.n_flat
+        stats = [saved[pos + 2 * i:pos + 2 * i + 2] for i in range(inner if normed else 0)]
+        pos += 2 * len(stats)
+        top = None
+        if not heads and not last_linear:
+            top, pos = saved[pos], pos + 1
+        params = saved[pos:]
+        grads = [None] * len(params)
+        need = ctx.needs_input_grad[2:]
+        dwg = GemmGroup()
+
+        def buffers(k):   # (dW, db) of parameter pair k: its .grad where it owns one (accumulated in place), else new zeros
+            dW, db = ctx.direct[2 * k], ctx.direct[2 * k + 1]
+            if dW is None or db is None:
+                dW, db = torch.zeros_like(params[2 * k]), torch.zeros_like(params[2 * k + 1])
+                grads[2 * k], grads[2 * k + 1] = dW, db
+            return dW, db
+
+        def weight_grad(k, i, g):   # layer pair k, reading input i
+            if not (need[2 * k] or need[2 * k + 1]):
+                return
+            src = keep[i][0]
+            dW, db = buffers(k)
+            if isinstance(src, Act8):
+                nk = 2 * (n + heads) + 2 * (i - 1)
+                norm = (*stats[i - 1], params[nk], params[nk + 1]) if normed and i > 0 else None
+                act8_bwd_weight_raw(g, src, dW, db, norm=norm)
+            else:
+                dwg.dw(g, src, dW, db)
+
+        def through_input(i, g):   # g = gradient of input i (the norm's output if there is one) -> of the layer in front, before act
+            a = keep[i][1]
+            if normed:
+                k = n + heads + i - 1
+                w = params[2 * k]
+                if need[2 * k] or need[2 * k + 1]:
+                    dw, db = buffers(k)
+                    return layer_norm_bwd_raw(g, a, w, *stats[i - 1], dw, db, leaky=True)[0]
+                return layer_norm_bwd_raw(g, a, w, *stats[i - 1], leaky=True)[0]
+            return act8_leaky_bwd_(g, a) if isinstance(a, Act8) else leaky_bwd_(g, a)
+
+        gs = [_c2d(g) for g in gs]
+        first = n - 1   # the highest trunk layer whose output gradient g is
+        if heads:
+            for j in range(heads):
+                weight_grad(n + j, n, gs[j])
+            if n == 0:
+                g = None
+                if ctx.needs_input_grad[0]:
+                    g = linear_bwd_input_raw(gs[0], params[0])
+                    for j in range(1, heads):
+                        g = linear_bwd_input_acc_raw(gs[j], params[2 * j], None, g)
+                dwg.launch()
+                return (g, None) + tuple(grads)
+            g = linear_bwd_input_raw(gs[0], params[2 * n])
+            for j in range(1, heads):
+                g = linear_bwd_input_acc_raw(gs[j], params[2 * (n + j)], None, g)
+            g = through_input(n, g)
+        else:
+            g = gs[0]
+            if top is not None:
+                g = leaky_bwd_(g.clone(), top)
+        for i in range(first, -1, -1):
+            weight_grad(i, i, g)
+            if i > 0:
+                g = through_input(i, linear_bwd_input_raw(g, params[2 * i]))
+            else:
+                g = linear_bwd_input_raw(g, params[0]) if ctx.needs_input_grad[0] else None
+        dwg.launch()
+        return (g, None) + tuple(grads)
+
+
+def _kept_stack(x, layers, heads, last_linear, norms, checkpoint, eps):
+    _check_checkpoint(checkpoint)
+    inner = len(layers) if heads else len(layers) - 1
+    if norms is not None and len(norms) != inner:
+        raise RuntimeError(f"{len(norms)} norms for {inner} hidden activations")
+    flat = []
+    for pair in list(layers) + list(heads) + list(norms or []):
+        flat += list(pair)
+    for w, b in norms or []:
+        if w is None or b is None:
+            raise ValueError("a stack's norms have a weight and a bias each")
+    train = torch.is_grad_enabled() and any(t.requires_grad for t in [x] + flat)
+    spec = (len(layers), len(heads), bool(last_linear), norms is not None, checkpoint, float(eps), train)
+    return _KeptStack.apply(x, spec, *flat)
 
 
 # ---------------------------------------------------------------- fused training-path operators (fewer, larger launches)
@@ -770,8 +1204,11 @@ def mlp_into(x, layers, out_buf, col0, grad_cols=None):
     return _MLPInto.apply(x, out_buf, int(col0), None if grad_cols is None else int(grad_cols), *flat)
 
 
-def mlp(x, layers, last_linear):
-    """layers: list of (weight [out,in], bias [out])."""
+def mlp(x, layers, last_linear, norms=None, checkpoint=None, norm_eps=1e-5):
+    """layers: list of (weight [out,in], bias [out]).  norms: one (weight, bias) per layer but the last - a layer norm behind its
+    activation; checkpoint = "e4m3": what the backward pass reads of the activations is kept in 8 bits (_KeptStack)"""
+    if norms is not None or checkpoint is not None:
+        return _kept_stack(x, layers, [], last_linear, norms, checkpoint, norm_eps)
     flat = []
     for W, b in layers:
         flat += [W, b]

@@ -334,7 +334,7 @@ class Trainer:
         nc = self.n_candidate
         return (self.n_neg, "given" if isinstance(nc, (tuple, list)) else nc, self.n_items, getattr(self.model, "TRAIN_RULE", "gt"),
                 getattr(self.model, "catalog_precision", None), getattr(self.model, "mlp_precision", None),
-                getattr(self.model, "gather_rows_bf16", None))
+                getattr(self.model, "gather_rows_bf16", None), getattr(self.model, "activation_checkpoint", None))
 
     def prepare_graph(self, s, r, u, row_offset=0):
         """Capture the hipGraph of a step for this batch shape now (no parameter update, no collective: two warm-up passes of
