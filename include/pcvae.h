@@ -450,7 +450,8 @@ int pcvae_layer_norm_bwd(const void* g, int64_t ldg, int type, int64_t M, int D,
  *     max |x| <= 448 * scale over the finite values, |x| held at 1.875 * 2^127); a code is the nearest OCP e4m3 multiple of it, ties to
  *     even; a positive value never becomes zero (it becomes the smallest code: LeakyReLU' reads off the codes exactly); NaN and +-inf
  *     become NaN.  codes [M, ldc], ldc a multiple of 16, >= 32 ceil(D / 32), 16-byte aligned, columns from D on hold code 0;
- *     scales [M, ldsc], ldsc a multiple of 4, >= 4 ceil(D / 128), 4-byte aligned, bytes from ceil(D / 32) on unused.
+ *     scales [ceil(M / 8)][ceil(D / 32)][8]: the bytes of 8 rows side by side, ldsc bytes per 8 rows (a multiple of 8, >= 8 ceil(D / 32)),
+ *     8-byte aligned; the bytes of rows from M on are neither written nor used.
  *     pack       : x -> codes, scales                         unpack : codes, scales -> y (the values, rounded to `type`)
  *     leaky_bwd  : g *= LeakyReLU'(x) in place, x the packed LeakyReLU output
  *     bwd_weight : dW[N, K] = sum_m g[m, n] q[m, k],  db[n] = sum_m g[m, n] (NULL: not wanted), q [M, K] the packed values; accumulate:

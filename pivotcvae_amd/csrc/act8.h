@@ -83,21 +83,46 @@ template <> struct RowType<_Float16> {
     }
 };
 
-// VW consecutive values of a row from column c on; columns from D on read 0 / are not written
+// ---- 16-byte pieces of a row of D columns, a lane's piece at column c (a multiple of VW) -------------------------------------------
+// How a row ends (template argument of the kernels, from row_end()):
+enum RowEnd {
+    ROW_FULL = 0,    // every lane's every piece lies inside the row
+    ROW_RAGGED = 1,  // pieces end anywhere; D >= VW: the last piece is the 16 bytes that END the row, moved down by the missing values -
+                     // one load per piece, whatever the width
+    ROW_TINY = 2     // D < VW: value by value
+};
 template <typename T>
-__device__ __forceinline__ void load_cols(const T* row, int c, int D, float (&v)[RowType<T>::VW]) {
+__device__ __forceinline__ Raw<16> piece_load(const T* row, int c, int D, int end) {
     constexpr int VW = RowType<T>::VW;
-    if (c + VW <= D) {
-        RowType<T>::widen(*reinterpret_cast<const Raw<16>*>(row + c), v);
-    } else {
+    if (end == ROW_TINY) return Raw<16>{};
+    return *reinterpret_cast<const Raw<16>*>(row + (end == ROW_FULL ? c : (c < D - VW ? c : D - VW)));
+}
+// the loaded piece's values; 0 from column D on.  last: this piece may hold the row's end (uniform over the lanes)
+template <typename T>
+__device__ __forceinline__ void piece_values(Raw<16> r, const T* row, int c, int D, int end, bool last, float (&v)[RowType<T>::VW]) {
+    constexpr int VW = RowType<T>::VW;
+    if (end == ROW_TINY) {
 #pragma unroll
         for (int i = 0; i < VW; ++i) v[i] = c + i < D ? RowType<T>::one(row + c + i) : 0.f;
+        return;
     }
+    if (end == ROW_RAGGED && last) {
+        const int missing = (VW - D % VW) % VW;   // uniform
+        Raw<16> m = r;
+        if (missing & (VW / 2)) m = Raw<16>{m.w[2], m.w[3], 0, 0};
+        if (missing & (VW / 4)) m = Raw<16>{m.w[1], m.w[2], m.w[3], 0};
+        if (VW == 8 && (missing & 1))
+            m = Raw<16>{__builtin_amdgcn_alignbit(m.w[1], m.w[0], 16), __builtin_amdgcn_alignbit(m.w[2], m.w[1], 16),
+                        __builtin_amdgcn_alignbit(m.w[3], m.w[2], 16), m.w[3] >> 16};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.w[i] = c + VW <= D ? r.w[i] : (c < D ? m.w[i] : 0u);
+    }
+    RowType<T>::widen(r, v);
 }
 template <typename T>
-__device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&v)[RowType<T>::VW]) {
+__device__ __forceinline__ void piece_store(T* row, int c, int D, int end, const float (&v)[RowType<T>::VW]) {
     constexpr int VW = RowType<T>::VW;
-    if (c + VW <= D) {
+    if (end == ROW_FULL || (end == ROW_RAGGED && c + VW <= D)) {
         Raw<16> r;
         RowType<T>::narrow(v, r);
         *reinterpret_cast<Raw<16>*>(row + c) = r;
@@ -106,6 +131,30 @@ __device__ __forceinline__ void store_cols(T* row, int c, int D, const float (&v
         for (int i = 0; i < VW; ++i)
             if (c + i < D) RowType<T>::put(row + c + i, v[i]);
     }
+}
+// VW fp32 parameters at a lane's columns; `none` without an array, 0 from column D on
+template <int VW>
+__device__ __forceinline__ void param_load(const float* p, int c, int D, int end, bool last, float none, float (&v)[VW]) {
+    if (!p) {
+#pragma unroll
+        for (int i = 0; i < VW; ++i) v[i] = end == ROW_FULL || c + i < D ? none : 0.f;
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < VW; h += 4) {
+        if (end == ROW_FULL || (D >= 4 && end == ROW_RAGGED)) {
+            float q[4];
+            piece_values<float>(piece_load<float>(p, c + h, D, end), p, c + h, D, end, last, q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[h + i] = q[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[h + i] = c + h + i < D ? p[c + h + i] : 0.f;
+        }
+    }
+}
+static inline int row_end(int D, int vw, int columns_of_all_lanes) {
+    return D < vw ? ROW_TINY : (D == columns_of_all_lanes ? ROW_FULL : ROW_RAGGED);
 }
 
 // ---- reductions over 2^k neighbouring lanes, every lane gets the result ------------------------------------------------------------
@@ -183,10 +232,17 @@ __device__ __forceinline__ void act8_values(uint32_t codes, float scale, float* 
     v[3] = b[1] * scale;
 }
 
+// where a block's scale byte lies: 8 rows side by side ([ceil(M / 8)][blocks][8 rows], ld bytes per 8 rows), so that the weight gradient's
+// lane - one block, 8 rows - reads its scales in one piece
+template <typename B>
+__device__ __forceinline__ B* act8_scale_at(B* scales, int64_t ld, int64_t row, int c) {
+    return scales + (row >> 3) * ld + (c / kAct8Block) * 8 + (row & 7);
+}
+
 // a lane's VW values at columns [c, c + VW) of a block it shares with its 32 / VW - 1 neighbours -> codes and (first lane) the scale byte.
 // Every lane of the block takes part, whatever its columns (values from D on are zeros); columns from D on get code 0.
 template <int VW>
-__device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, uint8_t* codes, uint8_t* scales) {
+__device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, uint8_t* codes, uint8_t* scale) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < VW; ++i) {
@@ -202,30 +258,13 @@ __device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, 
         } else {
             *reinterpret_cast<uint2*>(codes + c) = make_uint2(act8_codes(v, inv), act8_codes(v + 4, inv));
         }
-        if ((c & (kAct8Block - 1)) == 0) scales[c / kAct8Block] = (uint8_t)byte;
+        if ((c & (kAct8Block - 1)) == 0) *scale = (uint8_t)byte;
     }
 }
-// VW values of a row from its codes; 0 from Dp on (pad columns hold code 0)
-template <int VW>
-__device__ __forceinline__ void act8_load(const uint8_t* codes, const uint8_t* scales, int c, int Dp, float (&v)[VW]) {
-    if (c < Dp) {
-        const float s = act8_scale(scales[c / kAct8Block]);
-        if constexpr (VW == 4) {
-            act8_values(*reinterpret_cast<const uint32_t*>(codes + c), s, v);
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(codes + c);
-            act8_values(w.x, s, v);
-            act8_values(w.y, s, v + 4);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < VW; ++i) v[i] = 0.f;
-    }
-}
-
 // host: the types of a row
 static inline int row_type_size(int t) { return t == PCVAE_ROW_F32 ? 4 : 2; }
-// codes [M, ldc >= ceil(D / 32) * 32] at a multiple of 16 bytes, scale bytes [M, lds >= ceil(D / 128) * 4] at a multiple of 4 (error.cpp)
+// codes [M, ldc >= ceil(D / 32) * 32] at a multiple of 16 bytes, scale bytes [ceil(M / 8), lds >= 8 ceil(D / 32)] at a
+// multiple of 8 (error.cpp)
 int act8_check(const char* who, const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds, int64_t M, int64_t D);
 static inline bool row_type_ok(int t) { return t == PCVAE_ROW_F32 || t == PCVAE_ROW_BF16 || t == PCVAE_ROW_F16; }
 

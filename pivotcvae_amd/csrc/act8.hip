@@ -16,44 +16,78 @@ struct RowsParams {
     void* y; int64_t ldy;
     uint8_t* codes; int64_t ldc; uint8_t* scales; int64_t lds;
     int64_t M; int D, Dp;
-    unsigned pieces;   // lanes a row takes: Dp / VW
+    int pieces, end;              // lanes a row takes: Dp / VW;  RowEnd
+    int64_t step_rows; int step;  // the launch's lanes = step_rows rows + step pieces
 };
 
 enum { ROWS_PACK = 0, ROWS_UNPACK = 1, ROWS_LEAKY = 2 };
 
+// Lanes run along the rows back to back (a block's 8 or 4 lanes are neighbours: pieces is a multiple of them); a thread walks the launch's
+// stride in (row, piece) steps - one division per thread -, the next piece's loads in flight over the current one.
 template <typename T, int WHAT>
 __global__ __launch_bounds__(256) void act8_rows_kernel(RowsParams p) {
     constexpr int VW = RowType<T>::VW;
-    const int64_t total = p.M * p.pieces;   // a block's lanes (8 or 4) are neighbours: pieces is a multiple of them
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / p.pieces;
-        const int c = (int)(i - row * p.pieces) * VW;
+    const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    int64_t row = first / p.pieces;
+    int piece = (int)(first - row * p.pieces);
+    Raw<16> x{};
+    Raw<VW> q{};
+    uint32_t byte = 0;
+    auto load = [&](int64_t row, int c) {
+        if constexpr (WHAT == ROWS_PACK) x = piece_load<T>(static_cast<const T*>(p.x) + row * p.ldx, c, p.D, p.end);
+        if constexpr (WHAT == ROWS_LEAKY) x = piece_load<T>(static_cast<const T*>(p.y) + row * p.ldy, c, p.D, p.end);
+        if constexpr (WHAT != ROWS_PACK) {
+            q = *reinterpret_cast<const Raw<VW>*>(p.codes + row * p.ldc + c);
+            byte = *act8_scale_at(p.scales, p.lds, row, c);
+        }
+    };
+    if (row < p.M) load(row, piece * VW);
+    while (row < p.M) {
+        const int64_t r = row;
+        const int c = piece * VW;
+        const Raw<16> xr = x;
+        const Raw<VW> qr = q;
+        const float scale = act8_scale(byte);
+        row += p.step_rows;
+        piece += p.step;
+        if (piece >= p.pieces) {
+            piece -= p.pieces;
+            ++row;
+        }
+        if (row < p.M) load(row, piece * VW);
         float v[VW];
         if constexpr (WHAT == ROWS_PACK) {
-            load_cols(static_cast<const T*>(p.x) + row * p.ldx, c, p.D, v);
-            act8_store<VW>(v, c, p.Dp, p.codes + row * p.ldc, p.scales + row * p.lds);
+            piece_values<T>(xr, static_cast<const T*>(p.x) + r * p.ldx, c, p.D, p.end, true, v);
+            act8_store<VW>(v, c, p.Dp, p.codes + r * p.ldc, act8_scale_at(p.scales, p.lds, r, c));
         } else {
-            act8_load<VW>(p.codes + row * p.ldc, p.scales + row * p.lds, c, p.Dp, v);
-            T* y = static_cast<T*>(p.y) + row * p.ldy;
+            act8_values(qr.w[0], scale, v);
+            if constexpr (VW == 8) act8_values(qr.w[1], scale, v + 4);
+            T* y = static_cast<T*>(p.y) + r * p.ldy;
             if constexpr (WHAT == ROWS_LEAKY) {
                 float g[VW];
-                load_cols(y, c, p.D, g);
+                piece_values<T>(xr, y, c, p.D, p.end, true, g);
 #pragma unroll
                 for (int k = 0; k < VW; ++k) v[k] = v[k] > 0.f ? g[k] : kLeakySlope * g[k];
             }
-            store_cols(y, c, p.D, v);
+            piece_store<T>(y, c, p.D, p.end, v);
         }
     }
 }
+
+constexpr int kRowsGroups = 4096;
 
 template <int WHAT>
 int launch_rows(const char* what, int type, const RowsParams& p0, pcvae_stream_t stream) {
     RowsParams p = p0;
     if (p.M == 0) return PCVAE_OK;
     p.Dp = (int)cdiv(p.D, kAct8Block) * kAct8Block;
-    p.pieces = p.Dp / (type == PCVAE_ROW_F32 ? 4 : 8);
+    const int vw = type == PCVAE_ROW_F32 ? 4 : 8;
+    p.pieces = p.Dp / vw;
+    p.end = row_end(p.D, vw, p.Dp);
     const int64_t groups = cdiv(p.M * p.pieces, 256);
-    const dim3 grid((unsigned)(groups < 8192 ? groups : 8192));
+    const dim3 grid((unsigned)(groups < kRowsGroups ? groups : kRowsGroups));
+    p.step_rows = (int64_t)grid.x * 256 / p.pieces;
+    p.step = (int)((int64_t)grid.x * 256 % p.pieces);
     if (type == PCVAE_ROW_F32)
         hipLaunchKernelGGL((act8_rows_kernel<float, WHAT>), grid, dim3(256), 0, as_stream(stream), p);
     else if (type == PCVAE_ROW_BF16)
@@ -75,12 +109,14 @@ int check_plain_rows(const char* who, int type, int64_t M, int64_t D, int64_t ld
 // sum IS the fp32 value), three v_mfma_f32_32x32x16_bf16 per product, fp32 accumulate: fp32 products at a third of the bf16 rate.
 // fp16 g is exact in two components, bf16 g in one; behind a norm the factor g r_m is an fp32 number again (three).
 //
-// One workgroup: 128 (n) x 128 (k) of dW over a range of rows m, four waves of 64 x 64.  Both operands run ALONG the contraction in
-// memory's slow direction, so a chunk of 32 rows is turned on its way to LDS: a wave takes 8 consecutive rows, a lane holds the same
-// column of all 8 - which is the 16-byte operand piece of an MFMA.  LDS image of an operand: [4 pieces of 8 rows][128 columns][16 bytes]
-// (consecutive lanes, consecutive 16 bytes: no conflicts on either side).  Two stages, one barrier per chunk; the next chunk's loads are
-// in flight over the products.
-constexpr int TN = 128, TK = 128, TM = 32;
+// One workgroup: 128 (n) x 64 KT (k) of dW over a range of rows m, four waves of 64 x 32 KT.  Both operands run ALONG the contraction in
+// memory's slow direction, so a chunk of 32 rows is turned on its way to LDS: a wave takes 8 consecutive rows, a lane holds 2 (KT)
+// neighbouring columns of all 8, and a column's 8 values are the 16-byte operand piece of an MFMA.  LDS image of an operand:
+// [4 pieces of 8 rows][i][64 lanes][16 bytes], column = 2 lane + i (KT lane + i): consecutive lanes, consecutive 16 bytes on both sides (no
+// conflicts), and a wave whose MFMA tiles are the i of 32 lanes ends with KT neighbouring columns of dW per lane: wide stores.
+// Two stages, one barrier per chunk, the loads of two chunks in flight over the products.  Nothing in the loop is a scalar load: its
+// wait would be a wait for every LDS read too.
+constexpr int TN = 128, TM = 32;
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -90,8 +126,8 @@ struct DwParams {
     const float* mean; const float* rstd; const float* w; const float* b;   // the norm's, or null
     int64_t M; int N, K, Kp;
     int nn, nk, nz;            // tiles along n and k, ranges of m
-    int64_t m_per;             // rows of a range, a multiple of TM
-    float* part;               // [nz][nn nk][TN][TK] partial tiles (nz > 1), then [nz][nn TN] partial column sums
+    int64_t m_per;             // rows of a range, a multiple of 2 TM
+    float* part;               // nz > 1: [nz][nn nk][TN][TK] partial tiles, [nz][nn TN] partial column sums
     float* part_db;
     float* dW; int64_t lddw; float* db; int accumulate;
 };
@@ -124,11 +160,29 @@ __device__ __forceinline__ void split8(const float (&v)[8], uint4 (&c)[NC]) {
     }
 }
 
-template <typename T, int NC, bool NORM>
+// two neighbouring values of a gradient row
+template <typename T> struct Pair;
+template <> struct Pair<float> {
+    typedef Raw<8> raw;
+    static __device__ __forceinline__ float get(const raw& r, int i) { return __uint_as_float(r.w[i]); }
+    static __device__ __forceinline__ raw one(const float* p) { return raw{{__float_as_uint(*p), 0}}; }
+};
+template <> struct Pair<__bf16> {
+    typedef Raw<4> raw;
+    static __device__ __forceinline__ float get(const raw& r, int i) { return i ? high2(r.w[0]) : low2(r.w[0]); }
+    static __device__ __forceinline__ raw one(const __bf16* p) { return raw{{*reinterpret_cast<const uint16_t*>(p)}}; }
+};
+template <> struct Pair<_Float16> {
+    typedef Raw<4> raw;
+    static __device__ __forceinline__ float get(const raw& r, int i) { return (float)__builtin_bit_cast(f16x2_t, r.w[0])[i]; }
+    static __device__ __forceinline__ raw one(const _Float16* p) { return raw{{*reinterpret_cast<const uint16_t*>(p)}}; }
+};
+
+template <typename T, int NC, bool NORM, int KT>
 __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
-    __shared__ uint4 sA[2][NC][4][TN];
-    __shared__ uint4 sB[2][4][TK];
-    float (*sSum)[4][TN] = reinterpret_cast<float (*)[4][TN]>(&sA[0][0][0][0]);   // column sums, behind the last product
+    constexpr int TK = 64 * KT;
+    __shared__ uint4 sA0[NC][4][TN], sA1[NC][4][TN];
+    __shared__ uint4 sB0[4][TK], sB1[4][TK];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // logical order: all tiles of a range of rows next to each other (they share g and the codes in one XCD's L2)
     const int id = xcd_remap(blockIdx.x, gridDim.x);
@@ -136,177 +190,257 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
     const int64_t m0 = (int64_t)z * p.m_per, m1 = m0 + p.m_per < p.M ? m0 + p.m_per : p.M;
     const int chunks = (int)((m1 - m0 + TM - 1) / TM);
 
-    // columns past the end read the last one: their products land in rows / columns of dW that are never stored
-    const int na = min(tn * TN + lane, p.N - 1), nb = min(tn * TN + 64 + lane, p.N - 1);
-    const int kc = min(tk * TK + 2 * lane, p.Kp - 2);
-    const uint32_t sshift = 8 * ((kc >> 5) & 3);
+    // Columns past the end: the last pair of an odd N is loaded one column early (its second value is the real one: value i of a pair at
+    // n0 = N - 1 is column n0 + i - 1); whole pairs past N and codes past Kp read the last ones.  None of those reaches dW.
+    const int nc = min(tn * TN + 2 * lane, p.N - 2);
+    const int kc = min(tk * TK + KT * lane, p.Kp - KT);
     const T* g = static_cast<const T*>(p.g);
     const bool sums = NORM || (tk == 0 && p.db != nullptr);
 
-    float ga[8], gb[8], mr[NORM ? 8 : 1];
-    uint32_t q[8], sc[8];
-    float suma = 0.f, sumb = 0.f, muca = 0.f, mucb = 0.f;
+    struct Chunk {
+        typename Pair<T>::raw g[8];
+        uint32_t q[8];
+        uint2 s;
+        float r, mu;
+    } R0, R1;
+    float sum[2] = {0.f, 0.f}, muc[2] = {0.f, 0.f};
 
-    auto fetch = [&](int chunk) {
+    const uint32_t goff = (uint32_t)(nc < 0 ? 0 : nc) * (uint32_t)sizeof(T), qoff = (uint32_t)kc;
+    auto fetch = [&](int chunk, Chunk& c) {
         const int64_t base = m0 + (int64_t)chunk * TM + 8 * wave;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t m = base + j < m1 ? base + j : m1 - 1;
-            const T* gr = g + m * p.ldg;
-            ga[j] = RowType<T>::one(gr + na);
-            gb[j] = RowType<T>::one(gr + nb);
-            q[j] = *reinterpret_cast<const uint16_t*>(p.codes + m * p.ldc + kc);
-            sc[j] = *reinterpret_cast<const uint32_t*>(p.scales + m * p.lds + 4 * tk);
-            if constexpr (NORM) {
-                mr[j] = p.rstd[m];
-            }
-        }
-    };
-    auto place = [&](int chunk, int stage) {
-        const int64_t base = m0 + (int64_t)chunk * TM + 8 * wave;
-        if (base + 8 > m1) {   // rows from the range's end on count nothing
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (base + j >= m1) ga[j] = gb[j] = 0.f;
-        }
-        if (sums) {
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) s0 += ga[j], s1 += gb[j];
-            suma += s0;
-            sumb += s1;
-        }
-        if constexpr (NORM) {
-            float s0 = 0.f, s1 = 0.f;
+        if (base + 8 <= m1 && p.N > 1) {
+            const char* gr = reinterpret_cast<const char*>(g + base * p.ldg);
+            const uint8_t* qr = p.codes + base * p.ldc;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
+                c.g[j] = *reinterpret_cast<const typename Pair<T>::raw*>(gr + goff);
+                if constexpr (KT == 4) c.q[j] = *reinterpret_cast<const uint32_t*>(qr + qoff);
+                else c.q[j] = *reinterpret_cast<const uint16_t*>(qr + qoff);
+                gr += p.ldg * (int64_t)sizeof(T);
+                qr += p.ldc;
+            }
+        } else {   // the range's end; one column
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
                 const int64_t m = base + j < m1 ? base + j : m1 - 1;
-                const float mu = p.mean[m];
-                ga[j] *= mr[j];
-                gb[j] *= mr[j];
-                s0 = fmaf(ga[j], mu, s0);
-                s1 = fmaf(gb[j], mu, s1);
+                const char* gr = reinterpret_cast<const char*>(g + m * p.ldg);
+                const uint8_t* qr = p.codes + m * p.ldc;
+                typename Pair<T>::raw gv;
+                if (p.N > 1) gv = *reinterpret_cast<const typename Pair<T>::raw*>(gr + goff);
+                else gv = Pair<T>::one(reinterpret_cast<const T*>(gr));
+                uint32_t qv;
+                if constexpr (KT == 4) qv = *reinterpret_cast<const uint32_t*>(qr + qoff);
+                else qv = *reinterpret_cast<const uint16_t*>(qr + qoff);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {   // (no register is indexed by a variable)
+                    if (i == j) c.g[i] = gv, c.q[i] = qv;
+                }
             }
-            muca += s0;
-            mucb += s1;
         }
-        uint4 ca[NC], cb[NC];
-        split8<NC>(ga, ca);
-        split8<NC>(gb, cb);
-#pragma unroll
-        for (int k = 0; k < NC; ++k) {
-            sA[stage][k][wave][lane] = ca[k];
-            sA[stage][k][wave][64 + lane] = cb[k];
+        const int64_t group = (base < m1 ? base : m1 - 1) >> 3;   // base is a multiple of 8
+        c.s = *reinterpret_cast<const uint2*>(p.scales + group * p.lds + (kc >> 5) * 8);
+        if constexpr (NORM) {
+            const int64_t m = base + (lane & 7) < m1 ? base + (lane & 7) : m1 - 1;
+            c.r = p.rstd[m];
+            c.mu = p.mean[m];
         }
-        uint32_t lo[4], hi[4];
+    };
+    auto place = [&](int chunk, const Chunk& c, uint4 (&A)[NC][4][TN], uint4 (&B)[4][TK]) {
+        const int64_t base = m0 + (int64_t)chunk * TM + 8 * wave;
+        const int rows = m1 - base < 8 ? (int)(m1 - base) : 8;   // rows from the range's end on count nothing
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t e[2];
+        for (int i = 0; i < 2; ++i) {
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float s = act8_scale((sc[2 * j + i] >> sshift) & 0xffu);
-                e[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[2 * j + i], s, false));
+            for (int j = 0; j < 8; ++j) v[j] = Pair<T>::get(c.g[j], i);
+            if (rows < 8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = j < rows ? v[j] : 0.f;
             }
-            lo[j] = __builtin_amdgcn_perm(e[1], e[0], 0x05040100u);
-            hi[j] = __builtin_amdgcn_perm(e[1], e[0], 0x07060302u);
+            if (sums) sum[i] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            if constexpr (NORM) {
+                float t = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float r = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c.r), j));
+                    const float mu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c.mu), j));
+                    v[j] *= r;
+                    t = fmaf(v[j], mu, t);
+                }
+                muc[i] += t;
+            }
+            uint4 w[NC];
+            split8<NC>(v, w);
+#pragma unroll
+            for (int k = 0; k < NC; ++k) A[k][wave][64 * i + lane] = w[k];
         }
-        sB[stage][wave][2 * lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        sB[stage][wave][2 * lane + 1] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        uint32_t e[8][KT / 2];   // bf16 pairs (columns 2 h, 2 h + 1) of a row
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float s = act8_scale(((j < 4 ? c.s.x : c.s.y) >> (8 * (j & 3))) & 0xffu);
+            e[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.q[j], s, false));
+            if constexpr (KT == 4) e[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.q[j], s, true));
+        }
+        if (rows < 8) {   // (scale bytes behind the last row are not written)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int h = 0; h < KT / 2; ++h) e[j][h] = j < rows ? e[j][h] : 0u;
+        }
+#pragma unroll
+        for (int h = 0; h < KT / 2; ++h) {
+            B[wave][64 * (2 * h) + lane] =
+                make_uint4(__builtin_amdgcn_perm(e[1][h], e[0][h], 0x05040100u), __builtin_amdgcn_perm(e[3][h], e[2][h], 0x05040100u),
+                           __builtin_amdgcn_perm(e[5][h], e[4][h], 0x05040100u), __builtin_amdgcn_perm(e[7][h], e[6][h], 0x05040100u));
+            B[wave][64 * (2 * h + 1) + lane] =
+                make_uint4(__builtin_amdgcn_perm(e[1][h], e[0][h], 0x07060302u), __builtin_amdgcn_perm(e[3][h], e[2][h], 0x07060302u),
+                           __builtin_amdgcn_perm(e[5][h], e[4][h], 0x07060302u), __builtin_amdgcn_perm(e[7][h], e[6][h], 0x07060302u));
+        }
     };
 
-    const int wn = (wave >> 1) * 64, wk = (wave & 1) * 64;
-    f32x16_t acc[2][2];
+    const int hn = 32 * (wave >> 1), hk = 32 * (wave & 1), l = lane & 31;
+    f32x16_t acc[2][KT];
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < KT; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[a][b][i] = 0.f;
-
-    fetch(0);
-    place(0, 0);
-    if (chunks > 1) fetch(1);
-    __syncthreads();
-    for (int c = 0; c < chunks; ++c) {
-        const int stage = c & 1;
-        if (c + 1 < chunks) place(c + 1, stage ^ 1);
-        if (c + 2 < chunks) fetch(c + 2);
+    auto multiply = [&](uint4 (&A)[NC][4][TN], uint4 (&B)[4][TK]) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const int piece = 2 * s + (lane >> 5), l = lane & 31;
-            bf16x8_t b[2];
+            const int piece = 2 * s + (lane >> 5);
+            bf16x8_t b[KT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) b[t] = __builtin_bit_cast(bf16x8_t, sB[stage][piece][wk + 32 * t + l]);
+            for (int t = 0; t < KT; ++t) b[t] = __builtin_bit_cast(bf16x8_t, B[piece][64 * t + hk + l]);
 #pragma unroll
             for (int k = NC - 1; k >= 0; --k)   // the smallest components first
 #pragma unroll
                 for (int a = 0; a < 2; ++a) {
-                    const bf16x8_t av = __builtin_bit_cast(bf16x8_t, sA[stage][k][piece][wn + 32 * a + l]);
+                    const bf16x8_t av = __builtin_bit_cast(bf16x8_t, A[k][piece][64 * a + hn + l]);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) acc[a][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, b[t], acc[a][t], 0, 0, 0);
+                    for (int t = 0; t < KT; ++t) acc[a][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, b[t], acc[a][t], 0, 0, 0);
                 }
         }
+    };
+
+    // chunks in pairs, one per stage: a chunk behind the range's end is placed as zeros
+    fetch(0, R0);
+    fetch(1, R1);
+    place(0, R0, sA0, sB0);
+    fetch(2, R0);
+    __syncthreads();
+    for (int c = 0; c < chunks; c += 2) {
+        place(c + 1, R1, sA1, sB1);
+        fetch(c + 3, R1);
+        multiply(sA0, sB0);
+        __syncthreads();
+        place(c + 2, R0, sA0, sB0);
+        fetch(c + 4, R0);
+        multiply(sA1, sB1);
         __syncthreads();
     }
 
+    float (*sSum)[4][TN] = reinterpret_cast<float (*)[4][TN]>(&sA0[0][0][0]);   // column sums, behind the last product
     if (sums) {
-        sSum[0][wave][lane] = suma;
-        sSum[0][wave][64 + lane] = sumb;
-        if constexpr (NORM) {
-            sSum[1][wave][lane] = muca;
-            sSum[1][wave][64 + lane] = mucb;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sSum[0][wave][64 * i + lane] = sum[i];
+            if constexpr (NORM) sSum[1][wave][64 * i + lane] = muc[i];
         }
         __syncthreads();
     }
-    auto total = [&](int which, int n) { return (sSum[which][0][n] + sSum[which][1][n]) + (sSum[which][2][n] + sSum[which][3][n]); };
+    auto total = [&](int which, int at) { return (sSum[which][0][at] + sSum[which][1][at]) + (sSum[which][2][at] + sSum[which][3][at]); };
     if (tk == 0 && p.db != nullptr && threadIdx.x < TN) {
-        const int n = tn * TN + threadIdx.x;
-        const float t = total(0, threadIdx.x);
-        if (p.nz > 1) p.part_db[(int64_t)z * p.nn * TN + n] = t;
-        else if (n < p.N) p.db[n] = p.accumulate ? p.db[n] + t : t;
+        const int i = threadIdx.x >> 6, n0 = tn * TN + 2 * lane, n = n0 + i - (n0 == p.N - 1 && p.N > 1);
+        if (n >= n0 && n < p.N) {
+            const float t = total(0, threadIdx.x);
+            if (p.nz > 1) p.part_db[(int64_t)z * p.nn * TN + n] = t;
+            else p.db[n] = p.accumulate ? p.db[n] + t : t;
+        }
+    }
+    const int kk = KT * (hk + l), k = tk * TK + kk;   // KT neighbouring columns
+    float wv[KT], bv[KT];
+    if constexpr (NORM) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            wv[t] = p.w && k + t < p.K ? p.w[k + t] : 1.f;
+            bv[t] = p.b && k + t < p.K ? p.b[k + t] : 0.f;
+        }
     }
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int kk = wk + 32 * t + (lane & 31), k = tk * TK + kk;
-            const bool inside = k < p.K;
-            float wv = 1.f, bv = 0.f;
-            if constexpr (NORM) {
-                wv = p.w && inside ? p.w[k] : 1.f;
-                bv = p.b && inside ? p.b[k] : 0.f;
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int pair = hn + (i & 3) + 8 * (i >> 2) + 4 * (lane >> 5), n0 = tn * TN + 2 * pair;
+            const int n = n0 + a - (n0 == p.N - 1 && p.N > 1);
+            float v[KT];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int nr = wn + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * (lane >> 5), n = tn * TN + nr;
-                float v = acc[a][t][i];
-                if constexpr (NORM) v -= total(1, nr);
-                if constexpr (NORM) v = fmaf(wv, v, bv * total(0, nr));
-                if (p.nz > 1) {
-                    p.part[(((int64_t)z * tiles + tile) * TN + nr) * TK + kk] = v;
-                } else if (inside && n < p.N) {
-                    float* out = p.dW + (int64_t)n * p.lddw + k;
-                    *out = p.accumulate ? *out + v : v;
-                }
+            for (int t = 0; t < KT; ++t) v[t] = acc[a][t][i];
+            if constexpr (NORM) {
+                const float c0 = total(0, 64 * a + pair), c1 = total(1, 64 * a + pair);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) v[t] = fmaf(wv[t], v[t] - c1, bv[t] * c0);
+            }
+            if (n < n0 || n >= p.N) continue;
+            float* out = p.nz > 1 ? p.part + (((int64_t)z * tiles + tile) * TN + (n - tn * TN)) * TK + kk : p.dW + (int64_t)n * p.lddw + k;
+            const bool add = p.nz == 1 && p.accumulate;
+            if (p.nz > 1 || k + KT <= p.K) {
+                Raw<4 * KT> r;
+                if (add) r = *reinterpret_cast<const Raw<4 * KT>*>(out);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) r.w[t] = __float_as_uint(add ? __uint_as_float(r.w[t]) + v[t] : v[t]);
+                *reinterpret_cast<Raw<4 * KT>*>(out) = r;
+            } else {
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+                    if (k + t < p.K) out[t] = add ? out[t] + v[t] : v[t];
             }
         }
 }
 
-// the ranges of rows joined in order
-__global__ __launch_bounds__(256) void act8_weight_join_kernel(DwParams p) {
-    const int tiles = p.nn * p.nk;
-    const int64_t total = (int64_t)tiles * TN * TK / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int tile = (int)(i / (TN * TK / 4)), e = (int)(i % (TN * TK / 4)) * 4;
+// The ranges of rows joined: SL neighbouring runs of ranges per value, added in order (the same bits every run).  64 float4 of a tile per
+// SL threads; four ranges in flight per thread.
+template <int SL>
+__global__ __launch_bounds__(256) void act8_weight_join_kernel(DwParams p, int TK) {
+    __shared__ f32x4_t sh[256];
+    const int tiles = p.nn * p.nk, per_tile = TN * TK / 4, cols = 256 / SL;
+    const int64_t total = (int64_t)tiles * per_tile;
+    const int slice = threadIdx.x / cols, at = threadIdx.x % cols;
+    const int per = (p.nz + SL - 1) / SL, z0 = slice * per, z1 = z0 + per < p.nz ? z0 + per : p.nz;
+    for (int64_t i0 = (int64_t)blockIdx.x * cols; i0 < total; i0 += (int64_t)gridDim.x * cols) {   // total is a multiple of cols
+        const int64_t i = i0 + at;
+        const int tile = (int)(i / per_tile), e = (int)(i % per_tile) * 4;
         const int n = tile / p.nk * TN + e / TK, k = tile % p.nk * TK + e % TK;
-        if (n >= p.N || k >= p.K) continue;
+        const bool inside = n < p.N && k < p.K;
         f32x4_t s = {0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < p.nz; ++z)
-            s += *reinterpret_cast<const f32x4_t*>(p.part + ((int64_t)z * tiles + tile) * TN * TK + e);
-        float* out = p.dW + (int64_t)n * p.lddw + k;
+        if (inside) {
+            const float* q = p.part + (int64_t)tile * TN * TK + e;
+            const int64_t hop = (int64_t)tiles * TN * TK;
+            for (int z = z0; z < z1; z += 4) {
+                f32x4_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (k + j < p.K) out[j] = p.accumulate ? out[j] + s[j] : s[j];
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+                    if (z + j < z1) v[j] = *reinterpret_cast<const f32x4_t*>(q + (z + j) * hop);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s += v[j];
+            }
+        }
+        if constexpr (SL > 1) {
+            __syncthreads();
+            sh[threadIdx.x] = s;
+            __syncthreads();
+#pragma unroll
+            for (int j = 1; j < SL; ++j) s += sh[j * cols + at];   // (slice 0 keeps the sum of all)
+        }
+        if (slice == 0 && inside) {
+            float* out = p.dW + (int64_t)n * p.lddw + k;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (k + j < p.K) out[j] = p.accumulate ? out[j] + s[j] : s[j];
+        }
     }
     if (p.db) {
         for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < p.N; n += (int64_t)gridDim.x * 256) {
@@ -325,37 +459,51 @@ __global__ __launch_bounds__(256) void act8_weight_empty_kernel(DwParams p) {
     }
 }
 
-// ranges of rows: enough workgroups for two per CU, each at least 8 chunks long (a shorter range costs more in its partial tile than
-// it gives)
-struct DwPlan { int nn, nk, nz; int64_t m_per; };
+// tile width and ranges of rows
+struct DwPlan { int kt, nn, nk, nz; int64_t m_per; };
 DwPlan dw_plan(int64_t M, int64_t N, int64_t K) {
     DwPlan d;
+    d.kt = K > 128 ? 4 : 2;
     d.nn = (int)cdiv(N, TN);
-    d.nk = (int)cdiv(K, TK);
-    const int64_t tiles = (int64_t)d.nn * d.nk;
-    int64_t nz = tiles >= 512 ? 1 : 512 / tiles;
-    const int64_t most = cdiv(M, 8 * TM);
-    if (nz > most) nz = most;
-    if (nz < 1) nz = 1;
-    d.m_per = cdiv(cdiv(M, nz), TM) * TM;
+    d.nk = (int)cdiv(K, 64 * d.kt);
+    const int64_t tiles = (int64_t)d.nn * d.nk, chunks = cdiv(M, TM);
+    double best = 0.;
+    int64_t pick = 1;
+    for (int64_t nz = 1; nz <= 64 && nz * 2 <= chunks + 1; ++nz) {
+        const double rounds = (double)cdiv(tiles * nz, 512);
+        const double cost = rounds * ((double)cdiv(chunks, nz) + 4.) + (nz > 1 ? 6. + (double)tiles * nz * 64 * d.kt / (1 << 13) : 0.);
+        if (nz == 1 || cost < best) best = cost, pick = nz;
+    }
+    d.m_per = cdiv(cdiv(M, pick), 2 * TM) * 2 * TM;
     d.nz = (int)cdiv(M, d.m_per);
     return d;
 }
 size_t dw_ws(const DwPlan& d) {
-    return d.nz > 1 ? ((size_t)d.nz * d.nn * d.nk * TN * TK + (size_t)d.nz * d.nn * TN) * sizeof(float) : 0;
+    return d.nz > 1 ? ((size_t)d.nz * d.nn * d.nk * TN * 64 * d.kt + (size_t)d.nz * d.nn * TN) * sizeof(float) : 0;
 }
 
-template <typename T, int NC>
-int launch_dw(const DwParams& p, pcvae_stream_t stream) {
+template <typename T, int NC, int KT>
+void launch_dw_tile(const DwParams& p, pcvae_stream_t stream) {
     const dim3 grid((unsigned)(p.nn * p.nk * p.nz));
     if (p.mean)
-        hipLaunchKernelGGL((act8_weight_kernel<T, 3, true>), grid, dim3(256), 0, as_stream(stream), p);
+        hipLaunchKernelGGL((act8_weight_kernel<T, 3, true, KT>), grid, dim3(256), 0, as_stream(stream), p);
     else
-        hipLaunchKernelGGL((act8_weight_kernel<T, NC, false>), grid, dim3(256), 0, as_stream(stream), p);
+        hipLaunchKernelGGL((act8_weight_kernel<T, NC, false, KT>), grid, dim3(256), 0, as_stream(stream), p);
+}
+template <typename T, int NC>
+int launch_dw(const DwParams& p, int kt, pcvae_stream_t stream) {
+    if (kt == 4) launch_dw_tile<T, NC, 4>(p, stream);
+    else launch_dw_tile<T, NC, 2>(p, stream);
     if (int rc = check_launch("act8_bwd_weight")) return rc;
     if (p.nz == 1) return PCVAE_OK;
-    const int64_t groups = cdiv((int64_t)p.nn * p.nk * TN * TK / 4, 256);
-    hipLaunchKernelGGL(act8_weight_join_kernel, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, as_stream(stream), p);
+    const int64_t vecs = (int64_t)p.nn * p.nk * TN * 64 * kt / 4;
+    if (p.nz >= 8) {
+        const int64_t groups = cdiv(vecs, 32);
+        hipLaunchKernelGGL(act8_weight_join_kernel<8>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, as_stream(stream), p, 64 * kt);
+    } else {
+        const int64_t groups = cdiv(vecs, 256);
+        hipLaunchKernelGGL(act8_weight_join_kernel<1>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, as_stream(stream), p, 64 * kt);
+    }
     return check_launch("act8_bwd_weight (join)");
 }
 
@@ -417,8 +565,8 @@ extern "C" int pcvae_act8_bwd_weight(const void* g, int64_t ldg, int type, const
     }
     p.nn = d.nn; p.nk = d.nk; p.nz = d.nz; p.m_per = d.m_per;
     p.part = static_cast<float*>(ws);
-    p.part_db = need ? p.part + (size_t)d.nz * d.nn * d.nk * TN * TK : nullptr;
-    if (type == PCVAE_ROW_F32) return launch_dw<float, 3>(p, stream);
-    if (type == PCVAE_ROW_BF16) return launch_dw<__bf16, 1>(p, stream);
-    return launch_dw<_Float16, 2>(p, stream);
+    p.part_db = need ? p.part + (size_t)d.nz * d.nn * d.nk * TN * 64 * d.kt : nullptr;
+    if (type == PCVAE_ROW_F32) return launch_dw<float, 3>(p, d.kt, stream);
+    if (type == PCVAE_ROW_BF16) return launch_dw<__bf16, 1>(p, d.kt, stream);
+    return launch_dw<_Float16, 2>(p, d.kt, stream);
 }

@@ -145,8 +145,8 @@ int act8_check(const char* who, const uint8_t* codes, int64_t ldc, const uint8_t
     PCVAE_REQUIRE(codes && scales, "%s: null codes or scales", who);
     PCVAE_REQUIRE(ldc >= cdiv(D, kAct8Block) * kAct8Block && ldc % 16 == 0 && (uintptr_t)codes % 16 == 0,
                   "%s: codes need 16-byte aligned rows of at least %lld bytes", who, (long long)(cdiv(D, kAct8Block) * kAct8Block));
-    PCVAE_REQUIRE(lds >= cdiv(D, 4 * kAct8Block) * 4 && lds % 4 == 0 && (uintptr_t)scales % 4 == 0,
-                  "%s: scales need 4-byte aligned rows of at least %lld bytes", who, (long long)(cdiv(D, 4 * kAct8Block) * 4));
+    PCVAE_REQUIRE(lds >= cdiv(D, kAct8Block) * 8 && lds % 8 == 0 && (uintptr_t)scales % 8 == 0,
+                  "%s: scales need 8-byte aligned groups of at least %lld bytes per 8 rows", who, (long long)(cdiv(D, kAct8Block) * 8));
     return PCVAE_OK;
 }
 }  // namespace pcvae

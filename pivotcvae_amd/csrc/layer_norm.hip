@@ -65,41 +65,49 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[N][16], int 
     }
 }
 
-template <typename T, int TPR, int NV, bool KEEP>
+// the next row's loads are issued before the current row's sums: they are in flight over two reductions and the stores
+template <typename T, int TPR, int NV, int END, bool KEEP>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(FwdParams p) {
     constexpr int BLOCK = TPR > 256 ? TPR : 256, ROWS = BLOCK / TPR, VW = RowType<T>::VW;
     __shared__ float red0[2][1][16], red1[2][2][16];
     const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int tail = p.D / VW / TPR;   // the piece index the row's end falls into (pieces behind it are empty)
     float w[NV][VW], b[NV][VW];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = (k * TPR + lane) * VW;
-#pragma unroll
-        for (int i = 0; i < VW; ++i) {
-            w[k][i] = p.w && c + i < p.D ? p.w[c + i] : 1.f;
-            b[k][i] = p.b && c + i < p.D ? p.b[c + i] : 0.f;
-        }
+        param_load<VW>(p.w, c, p.D, END, k >= tail, 1.f, w[k]);
+        param_load<VW>(p.b, c, p.D, END, k >= tail, 0.f, b[k]);
     }
-    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.M; row0 += (int64_t)gridDim.x * ROWS) {
+    const T* x = static_cast<const T*>(p.x);
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    auto row_at = [&](int64_t row0) { return x + (row0 + sub < p.M ? row0 + sub : p.M - 1) * p.ldx; };
+    Raw<16> next[NV];
+    int64_t row0 = (int64_t)blockIdx.x * ROWS;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) next[k] = piece_load<T>(row_at(row0), (k * TPR + lane) * VW, p.D, END);
+    for (; row0 < p.M; row0 += step) {
         const bool live = row0 + sub < p.M;
         const int64_t row = live ? row0 + sub : p.M - 1;
-        const T* xr = static_cast<const T*>(p.x) + row * p.ldx;
-        float v[NV][VW], s[1] = {0.f};
+        float v[NV][VW], s[1] = {0.f}, m[2] = {0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < NV; ++k) load_cols(xr, (k * TPR + lane) * VW, p.D, v[k]);
+        for (int k = 0; k < NV; ++k) piece_values<T>(next[k], row_at(row0), (k * TPR + lane) * VW, p.D, END, k >= tail, v[k]);
+        if (row0 + step < p.M) {
+#pragma unroll
+            for (int k = 0; k < NV; ++k) next[k] = piece_load<T>(row_at(row0 + step), (k * TPR + lane) * VW, p.D, END);
+        }
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int i = 0; i < VW; ++i) s[0] += v[k][i];
         row_sum<TPR, 1>(s, red0, 0);
         const float near = s[0] / p.D;
-        float m[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + lane) * VW;
 #pragma unroll
             for (int i = 0; i < VW; ++i) {
-                const float d = c + i < p.D ? v[k][i] - near : 0.f;
+                const float d = END == ROW_FULL || c + i < p.D ? v[k][i] - near : 0.f;
                 m[0] += d;
                 m[1] = fmaf(d, d, m[1]);
             }
@@ -117,47 +125,78 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(F
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + lane) * VW;
-            if constexpr (KEEP)
-                act8_store<VW>(v[k], c, p.Dp, p.codes + row * p.ldc, p.scales + row * p.lds);
+            if constexpr (KEEP) act8_store<VW>(v[k], c, p.Dp, p.codes + row * p.ldc, act8_scale_at(p.scales, p.lds, row, c));
             float o[VW];
 #pragma unroll
             for (int i = 0; i < VW; ++i) o[i] = fmaf((v[k][i] - mean) * rstd, w[k][i], b[k][i]);
-            store_cols(yr, c, p.D, o);
+            piece_store<T>(yr, c, p.D, END, o);
         }
     }
 }
 
-template <typename T, int TPR, int NV, bool KEPT>
+template <typename T, int TPR, int NV, int END, bool KEPT>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(BwdParams p) {
     constexpr int BLOCK = TPR > 256 ? TPR : 256, ROWS = BLOCK / TPR, VW = RowType<T>::VW;
     __shared__ float red[2][2][16];
     const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int tail = p.D / VW / TPR;
     float w[NV][VW], dw[NV][VW], db[NV][VW];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int c = (k * TPR + lane) * VW;
+        param_load<VW>(p.w, (k * TPR + lane) * VW, p.D, END, k >= tail, 1.f, w[k]);
 #pragma unroll
-        for (int i = 0; i < VW; ++i) {
-            w[k][i] = c + i < p.D ? (p.w ? p.w[c + i] : 1.f) : 0.f;
-            dw[k][i] = db[k][i] = 0.f;
-        }
+        for (int i = 0; i < VW; ++i) dw[k][i] = db[k][i] = 0.f;
     }
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    auto row_of = [&](int64_t row0) { return row0 + sub < p.M ? row0 + sub : p.M - 1; };
+    struct Loaded {
+        Raw<16> g[NV], x[KEPT ? 1 : NV];
+        Raw<VW> q[KEPT ? NV : 1];
+        uint32_t s[KEPT ? NV : 1];
+        float mean, rstd;
+    } next;
+    auto load = [&](int64_t row0) {
+        const int64_t row = row_of(row0);
+        next.mean = p.mean[row];
+        next.rstd = p.rstd[row];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int c = (k * TPR + lane) * VW;
+            next.g[k] = piece_load<T>(static_cast<const T*>(p.g) + row * p.ldg, c, p.D, END);
+            if constexpr (KEPT) {
+                const int cc = c < p.Dp ? c : p.Dp - VW;
+                next.q[k] = *reinterpret_cast<const Raw<VW>*>(p.codes + row * p.ldc + cc);
+                next.s[k] = *act8_scale_at(p.scales, p.lds, row, cc);
+            } else {
+                next.x[k] = piece_load<T>(static_cast<const T*>(p.x) + row * p.ldx, c, p.D, END);
+            }
+        }
+    };
     int slot = 0;
-    for (int64_t row0 = (int64_t)blockIdx.x * ROWS; row0 < p.M; row0 += (int64_t)gridDim.x * ROWS) {
+    int64_t row0 = (int64_t)blockIdx.x * ROWS;
+    load(row0);
+    for (; row0 < p.M; row0 += step) {
         const bool live = row0 + sub < p.M;
-        const int64_t row = live ? row0 + sub : p.M - 1;
-        const T* gr = static_cast<const T*>(p.g) + row * p.ldg;
-        const float mean = p.mean[row], rstd = p.rstd[row];
+        const int64_t row = row_of(row0);
+        const float mean = next.mean, rstd = next.rstd;
         float x[NV][VW], g[NV][VW], s[2] = {0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + lane) * VW;
-            load_cols(gr, c, p.D, g[k]);
-            if constexpr (KEPT)
-                act8_load<VW>(p.codes + row * p.ldc, p.scales + row * p.lds, c, p.Dp, x[k]);
-            else
-                load_cols(static_cast<const T*>(p.x) + row * p.ldx, c, p.D, x[k]);
+            piece_values<T>(next.g[k], static_cast<const T*>(p.g) + row * p.ldg, c, p.D, END, k >= tail, g[k]);
+            if constexpr (KEPT) {
+                const float scale = act8_scale(next.s[k]);   // columns behind the row read its last codes: their g and w are 0
+                act8_values(next.q[k].w[0], scale, x[k]);
+                if constexpr (VW == 8) act8_values(next.q[k].w[1], scale, x[k] + 4);
+                if (END != ROW_FULL && c >= p.Dp) {
+#pragma unroll
+                    for (int i = 0; i < VW; ++i) x[k][i] = 0.f;
+                }
+            } else {
+                piece_values<T>(next.x[k], static_cast<const T*>(p.x) + row * p.ldx, c, p.D, END, k >= tail, x[k]);
+            }
         }
+        if (row0 + step < p.M) load(row0 + step);
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -185,22 +224,22 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(B
                 o[i] = rstd * (fmaf(w[k][i], g[k][i], -c0) - h * c1);
                 if (p.leaky && !(x[k][i] > 0.f)) o[i] *= kLeakySlope;
             }
-            store_cols(dr, c, p.D, o);
+            piece_store<T>(dr, c, p.D, END, o);
         }
     }
     // the workgroup's partial row of (dw, db): rows of a workgroup that share columns meet in LDS, in row order
     float* part = p.part + (int64_t)blockIdx.x * 2 * p.D;
     if constexpr (ROWS == 1) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int c = (k * TPR + lane) * VW;
-            store_cols(part, c, p.D, reinterpret_cast<const float(&)[4]>(dw[k][0]));
-            store_cols(part + p.D, c, p.D, reinterpret_cast<const float(&)[4]>(db[k][0]));
-            if constexpr (VW == 8) {
-                store_cols(part, c + 4, p.D, reinterpret_cast<const float(&)[4]>(dw[k][4]));
-                store_cols(part + p.D, c + 4, p.D, reinterpret_cast<const float(&)[4]>(db[k][4]));
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int h = 0; h < VW; h += 4) {
+                const int c = (k * TPR + lane) * VW + h;
+                const float a[4] = {dw[k][h], dw[k][h + 1], dw[k][h + 2], dw[k][h + 3]};
+                const float e[4] = {db[k][h], db[k][h + 1], db[k][h + 2], db[k][h + 3]};
+                piece_store<float>(part, c, p.D, END, a);
+                piece_store<float>(part + p.D, c, p.D, END, e);
             }
-        }
     } else {
         __shared__ float join[ROWS > 1 ? BLOCK * VW : 1];   // one piece of every thread at a time: [sub][TPR * VW columns]
 #pragma unroll
@@ -223,54 +262,79 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_bwd_kernel(B
     }
 }
 
-// out[c] (+)= sum over the G partial rows: 64 columns per workgroup, 16 runs of rows side by side, joined in order
+// out[c] (+)= sum over the G partial rows: 32 columns per workgroup, 32 runs of rows side by side (eight rows of a run in flight), the runs
+// joined in order
 __global__ __launch_bounds__(1024) void column_join_kernel(const float* part, int G, int D, float* dw, float* db, int accumulate) {
-    __shared__ float s[16][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), run = threadIdx.x >> 6;
-    const int per = (G + 15) / 16, g0 = run * per, g1 = g0 + per < G ? g0 + per : G;
+    __shared__ float s[32][33];
+    const int col = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
+    const int per = (G + 31) / 32, g0 = run * per, g1 = g0 + per < G ? g0 + per : G;
     float t = 0.f;
-    if (c < 2 * D)
-        for (int g = g0; g < g1; ++g) t += part[(int64_t)g * 2 * D + c];
-    s[run][threadIdx.x & 63] = t;
+    if (c < 2 * D) {
+        const float* q = part + c;
+        for (int g = g0; g < g1; g += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = g + i < g1 ? q[(int64_t)(g + i) * 2 * D] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t += v[i];
+        }
+    }
+    s[run][col] = t;
     __syncthreads();
     if (run == 0 && c < 2 * D) {
 #pragma unroll
-        for (int r = 1; r < 16; ++r) t += s[r][threadIdx.x];
+        for (int r = 1; r < 32; ++r) t += s[r][col];
         float* out = c < D ? (dw ? dw + c : nullptr) : (db ? db + (c - D) : nullptr);
         if (out) *out = accumulate ? *out + t : t;
     }
 }
 
-// threads per row and 16-byte pieces per thread for a width: the fewest threads that cover the row with one piece each up to a wave,
-// then up to 4 pieces per lane of a wave (no barrier), 256 threads, 1024 threads
-struct Plan { int tpr, nv; };
+// threads per row and 16-byte pieces per thread for a width: one piece each up to a wave, then more pieces per lane of a wave (no barrier)
+// as far as the registers of the backward go - it holds w, dw, db in fp32 per column: 4 pieces of fp32, 2 of the half types -, then 256
+// threads, then 1024
+struct Plan { int tpr, nv, end; };
 Plan plan(int D, int vw) {
     const int pieces = (int)cdiv(D, vw);
-    if (pieces <= 8) return {8, 1};
-    if (pieces <= 16) return {16, 1};
-    if (pieces <= 32) return {32, 1};
-    if (pieces <= 64) return {64, 1};
-    if (pieces <= 128) return {64, 2};
-    if (pieces <= 256) return {64, 4};
-    if (pieces <= 512) return {256, 2};
-    if (pieces <= 1024) return {256, 4};
-    if (pieces <= 2048) return {1024, 2};
-    return {1024, 4};
+    Plan pl{1024, vw == 4 ? 4 : 2, 0};
+    const int few[4] = {8, 16, 32, 64};
+    for (int t : few)
+        if (pieces <= t) { pl = {t, 1, 0}; break; }
+    if (pieces > 64) {
+        if (pieces <= 128) pl = {64, 2, 0};
+        else if (pieces <= 256 && vw == 4) pl = {64, 4, 0};
+        else if (pieces <= 256) pl = {256, 1, 0};
+        else if (pieces <= 512) pl = {256, 2, 0};
+        else if (pieces <= 1024 && vw == 4) pl = {256, 4, 0};
+        else if (pieces <= 1024) pl = {1024, 1, 0};
+        else if (pieces <= 2048) pl = {1024, 2, 0};
+    }
+    pl.end = row_end(D, vw, pl.tpr * pl.nv * vw);
+    return pl;
 }
 
-template <typename F>
+template <int VW, typename F>
 int with_plan(const Plan& pl, F f) {
-#define PCVAE_LN_PLAN(t, n) if (pl.tpr == t && pl.nv == n) return f(std::integral_constant<int, t>{}, std::integral_constant<int, n>{})
-    PCVAE_LN_PLAN(8, 1);
-    PCVAE_LN_PLAN(16, 1);
-    PCVAE_LN_PLAN(32, 1);
-    PCVAE_LN_PLAN(64, 1);
-    PCVAE_LN_PLAN(64, 2);
-    PCVAE_LN_PLAN(64, 4);
-    PCVAE_LN_PLAN(256, 2);
-    PCVAE_LN_PLAN(256, 4);
-    PCVAE_LN_PLAN(1024, 2);
-    PCVAE_LN_PLAN(1024, 4);
+#define PCVAE_LN_PLAN(t, n)                                                                                                          \
+    if (pl.tpr == t && pl.nv == n) {                                                                                                 \
+        if (pl.end == ROW_FULL) return f(std::integral_constant<int, t>{}, std::integral_constant<int, n>{}, std::integral_constant<int, 0>{}); \
+        return f(std::integral_constant<int, t>{}, std::integral_constant<int, n>{}, std::integral_constant<int, 1>{});              \
+    }
+    if (pl.end == ROW_TINY) return f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{}, std::integral_constant<int, 2>{});
+    PCVAE_LN_PLAN(8, 1)
+    PCVAE_LN_PLAN(16, 1)
+    PCVAE_LN_PLAN(32, 1)
+    PCVAE_LN_PLAN(64, 1)
+    PCVAE_LN_PLAN(64, 2)
+    PCVAE_LN_PLAN(256, 2)
+    PCVAE_LN_PLAN(1024, 2)
+    if constexpr (VW == 4) {
+        PCVAE_LN_PLAN(64, 4)
+        PCVAE_LN_PLAN(256, 4)
+        PCVAE_LN_PLAN(1024, 4)
+    } else {
+        PCVAE_LN_PLAN(256, 1)
+        PCVAE_LN_PLAN(1024, 1)
+    }
 #undef PCVAE_LN_PLAN
     set_error("layer_norm: no plan");
     return PCVAE_EINVAL;
@@ -317,13 +381,13 @@ extern "C" int pcvae_layer_norm_fwd(const void* x, int64_t ldx, int type, int64_
     const unsigned grid = (unsigned)(groups < 2048 ? groups : 2048);
     return with_type(type, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return with_plan(pl, [&](auto t, auto n) {
-            constexpr int TPR = decltype(t)::value, NV = decltype(n)::value;
+        return with_plan<RowType<T>::VW>(pl, [&](auto t, auto n, auto e) {
+            constexpr int TPR = decltype(t)::value, NV = decltype(n)::value, END = decltype(e)::value;
             const dim3 block(TPR > 256 ? TPR : 256);
             if (codes)
-                hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV, true>), dim3(grid), block, 0, as_stream(stream), p);
+                hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV, END, true>), dim3(grid), block, 0, as_stream(stream), p);
             else
-                hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV, false>), dim3(grid), block, 0, as_stream(stream), p);
+                hipLaunchKernelGGL((layer_norm_fwd_kernel<T, TPR, NV, END, false>), dim3(grid), block, 0, as_stream(stream), p);
             return check_launch("layer_norm_fwd");
         });
     });
@@ -366,18 +430,18 @@ extern "C" int pcvae_layer_norm_bwd(const void* g, int64_t ldg, int type, int64_
                 (int)cdiv(D, kAct8Block) * kAct8Block, leaky, 1.f / D};
     const int rc = with_type(type, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
-        return with_plan(pl, [&](auto t, auto n) {
-            constexpr int TPR = decltype(t)::value, NV = decltype(n)::value;
+        return with_plan<RowType<T>::VW>(pl, [&](auto t, auto n, auto e) {
+            constexpr int TPR = decltype(t)::value, NV = decltype(n)::value, END = decltype(e)::value;
             const dim3 block(TPR > 256 ? TPR : 256);
             if (codes)
-                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, TPR, NV, true>), dim3(G), block, 0, as_stream(stream), p);
+                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, TPR, NV, END, true>), dim3(G), block, 0, as_stream(stream), p);
             else
-                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, TPR, NV, false>), dim3(G), block, 0, as_stream(stream), p);
+                hipLaunchKernelGGL((layer_norm_bwd_kernel<T, TPR, NV, END, false>), dim3(G), block, 0, as_stream(stream), p);
             return check_launch("layer_norm_bwd");
         });
     });
     if (rc != PCVAE_OK || (!dweight && !dbias)) return rc;
-    hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)cdiv(2 * D, 64)), dim3(1024), 0, as_stream(stream), p.part, G, D, dweight, dbias,
+    hipLaunchKernelGGL(column_join_kernel, dim3((unsigned)cdiv(2 * D, 32)), dim3(1024), 0, as_stream(stream), p.part, G, D, dweight, dbias,
                        accumulate);
     return check_launch("layer_norm_bwd (column sums)");
 }

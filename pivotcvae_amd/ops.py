@@ -559,7 +559,7 @@ class Act8:
             raise TypeError("Act8: codes and scales are uint8")
         if D < 1:
             raise ValueError("Act8: width 0")
-        if tuple(codes.shape) != (M, self.code_width(D)) or tuple(scales.shape) != (M, self.scale_width(D)):
+        if tuple(codes.shape) != (M, self.code_width(D)) or tuple(scales.shape) != (-(-M // 8), self.scale_width(D)):
             raise RuntimeError(f"Act8: codes {tuple(codes.shape)} / scales {tuple(scales.shape)} do not hold {tuple(shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise ValueError("Act8: codes and scales are contiguous")
@@ -570,14 +570,14 @@ class Act8:
         return -(-D // ACT8_BLOCK) * ACT8_BLOCK
 
     @staticmethod
-    def scale_width(D):
-        return -(-D // (4 * ACT8_BLOCK)) * 4
+    def scale_width(D):   # bytes per 8 rows: their scales side by side
+        return -(-D // ACT8_BLOCK) * 8
 
     @classmethod
     def empty(cls, shape, dtype, device):
         M, D = torch.Size(shape[:-1]).numel(), shape[-1]
         return cls(torch.empty(M, cls.code_width(D), dtype=torch.uint8, device=device),
-                   torch.empty(M, cls.scale_width(D), dtype=torch.uint8, device=device), shape, dtype)
+                   torch.empty(-(-M // 8), cls.scale_width(D), dtype=torch.uint8, device=device), shape, dtype)
 
     @property
     def device(self):

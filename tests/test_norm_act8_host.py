@@ -28,15 +28,15 @@ def bwd(**kw):
 @pytest.mark.parametrize("kw,say", [(dict(type=3), "type"), (dict(M=-1), "rows"), (dict(D=0), "width"), (dict(D=16385, ldx=16385), "width"),
                                     (dict(x=None), "null"), (dict(y=None), "null"), (dict(ldx=63), "stride"), (dict(ldy=63), "stride"),
                                     (dict(eps=-1.0), "eps"), (dict(codes=P), "together"), (dict(scales=P), "together"),
-                                    (dict(codes=P, scales=P, ldc=32, lds=4), "codes"), (dict(codes=P + 8, scales=P, ldc=64, lds=4), "codes"),
-                                    (dict(codes=P, scales=P + 2, ldc=64, lds=4), "scales"), (dict(codes=P, scales=P, ldc=64, lds=2), "scales"),
-                                    (dict(codes=P, scales=P, ldc=72, lds=4), "codes")])
+                                    (dict(codes=P, scales=P, ldc=32, lds=16), "codes"), (dict(codes=P + 8, scales=P, ldc=64, lds=16), "codes"),
+                                    (dict(codes=P, scales=P + 4, ldc=64, lds=16), "scales"), (dict(codes=P, scales=P, ldc=64, lds=8), "scales"),
+                                    (dict(codes=P, scales=P, ldc=72, lds=16), "codes")])
 def test_layer_norm_forward_refuses(kw, say):
     assert fwd(**kw) == -1 and say in text()
 
 
 @pytest.mark.parametrize("kw,say", [(dict(type=-1), "type"), (dict(D=0), "width"), (dict(g=None), "null"), (dict(dx=None), "null"), (dict(x=None), "either"),
-                                    (dict(codes=P, scales=P, ldc=64, lds=4), "either"), (dict(mean=None), "mean"), (dict(rstd=None), "mean"),
+                                    (dict(codes=P, scales=P, ldc=64, lds=16), "either"), (dict(mean=None), "mean"), (dict(rstd=None), "mean"),
                                     (dict(ldg=1), "stride"), (dict(lddx=8), "stride"), (dict(ldx=8), "stride")])
 def test_layer_norm_backward_refuses(kw, say):
     assert bwd(**kw) == -1 and say in text()
@@ -48,28 +48,28 @@ def test_workspaces_are_checked():
     assert _hip.lib().pcvae_layer_norm_bwd_ws_bytes(0, 64, 0) == 0 and _hip.lib().pcvae_layer_norm_bwd_ws_bytes(4, 0, 0) == 0
     need = _hip.lib().pcvae_act8_bwd_weight_ws_bytes(8192, 256, 1419)
     assert need > 0
-    a = [P, 256, 0, P, 1440, P, 48, 8192, 256, 1419, None, None, None, None, P, 1419, P, 0]
+    a = [P, 256, 0, P, 1440, P, 360, 8192, 256, 1419, None, None, None, None, P, 1419, P, 0]
     assert _hip.lib().pcvae_act8_bwd_weight(*a, P, need - 1, None) == -3 and "workspace" in text()
     assert _hip.lib().pcvae_act8_bwd_weight(*a, None, need, None) == -3
 
 
-@pytest.mark.parametrize("at,value,say", [(2, 9, "type"), (0, None, "null"), (1, 255, "stride"), (3, None, "null"), (4, 1424, "codes"), (6, 44, "scales"),
+@pytest.mark.parametrize("at,value,say", [(2, 9, "type"), (0, None, "null"), (1, 255, "stride"), (3, None, "null"), (4, 1424, "codes"), (6, 352, "scales"),
                                           (8, 0, "N"), (9, 0, "width"), (10, P, "together"), (12, P, "mean"), (14, None, "dW"), (15, 1418, "stride"),
                                           (7, -1, "rows")])
 def test_weight_gradient_refuses(at, value, say):
-    a = [P, 256, 0, P, 1440, P, 48, 8192, 256, 1419, None, None, None, None, P, 1419, P, 0]
+    a = [P, 256, 0, P, 1440, P, 360, 8192, 256, 1419, None, None, None, None, P, 1419, P, 0]
     a[at] = value
     assert _hip.lib().pcvae_act8_bwd_weight(*a, P, 1 << 40, None) == -1 and say in text()
 
 
 def test_rows_kernels_refuse():
     L = _hip.lib()
-    assert L.pcvae_act8_pack(P, 64, 0, 4, 64, None, 64, P, 4, None) == -1 and "null" in text()
-    assert L.pcvae_act8_pack(None, 64, 0, 4, 64, P, 64, P, 4, None) == -1
-    assert L.pcvae_act8_pack(P, 60, 0, 4, 64, P, 64, P, 4, None) == -1 and "stride" in text()
-    assert L.pcvae_act8_pack(P, 64, 7, 4, 64, P, 64, P, 4, None) == -1 and "type" in text()
-    assert L.pcvae_act8_unpack(P, 32, P, 4, 4, 64, P, 64, 0, None) == -1 and "codes" in text()
-    assert L.pcvae_act8_leaky_bwd(P, 3, 0, P, 64, P, 4, 4, 64, None) == -1 and "stride" in text()
+    assert L.pcvae_act8_pack(P, 64, 0, 4, 64, None, 64, P, 16, None) == -1 and "null" in text()
+    assert L.pcvae_act8_pack(None, 64, 0, 4, 64, P, 64, P, 16, None) == -1
+    assert L.pcvae_act8_pack(P, 60, 0, 4, 64, P, 64, P, 16, None) == -1 and "stride" in text()
+    assert L.pcvae_act8_pack(P, 64, 7, 4, 64, P, 64, P, 16, None) == -1 and "type" in text()
+    assert L.pcvae_act8_unpack(P, 32, P, 16, 4, 64, P, 64, 0, None) == -1 and "codes" in text()
+    assert L.pcvae_act8_leaky_bwd(P, 3, 0, P, 64, P, 16, 4, 64, None) == -1 and "stride" in text()
     assert L.pcvae_act8_pack(None, 0, 0, 0, 64, None, 0, None, 0, None) == 0   # no rows: nothing to do
 
 
@@ -87,7 +87,7 @@ def test_python_layer_refuses():
     with pytest.raises(ValueError, match="weight and a bias"):
         ops.mlp_heads(x, [(x, x[0])], (x, x[0]), (x, x[0]), norms=[(None, None)])
     u8 = torch.zeros(4, 64, dtype=torch.uint8)
-    sc = torch.zeros(4, 4, dtype=torch.uint8)
+    sc = torch.zeros(1, 16, dtype=torch.uint8)
     assert ops.Act8(u8, sc, (4, 64)).nbytes == 4 * 64 + 16 and ops.Act8(u8, sc, (2, 2, 50)).shape == (2, 2, 50)
     with pytest.raises(RuntimeError, match="do not hold"):
         ops.Act8(u8, sc, (4, 65))
