@@ -188,7 +188,6 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
     const int id = xcd_remap(blockIdx.x, gridDim.x);
     const int tiles = p.nn * p.nk, z = id / tiles, tile = id % tiles, tn = tile / p.nk, tk = tile % p.nk;
     const int64_t m0 = (int64_t)z * p.m_per, m1 = m0 + p.m_per < p.M ? m0 + p.m_per : p.M;
-    const int chunks = (int)((m1 - m0 + TM - 1) / TM);
 
     // Columns past the end: the last pair of an odd N is loaded one column early (its second value is the real one: value i of a pair at
     // n0 = N - 1 is column n0 + i - 1); whole pairs past N and codes past Kp read the last ones.  None of those reaches dW.
@@ -202,75 +201,84 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
         uint32_t q[8];
         uint2 s;
         float r, mu;
-    } R0, R1;
+    };
     float sum[2] = {0.f, 0.f}, muc[2] = {0.f, 0.f};
-
     const uint32_t goff = (uint32_t)(nc < 0 ? 0 : nc) * (uint32_t)sizeof(T), qoff = (uint32_t)kc;
-    auto fetch = [&](int chunk, Chunk& c) {
-        const int64_t base = m0 + (int64_t)chunk * TM + 8 * wave;
-        if (base + 8 <= m1 && p.N > 1) {
-            const char* gr = reinterpret_cast<const char*>(g + base * p.ldg);
-            const uint8_t* qr = p.codes + base * p.ldc;
+
+    // this wave's 8 rows from m on, all inside the range
+    auto fetch = [&](int64_t m, Chunk& c) {
+        const char* gr = reinterpret_cast<const char*>(g + m * p.ldg);
+        const uint8_t* qr = p.codes + m * p.ldc;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                c.g[j] = *reinterpret_cast<const typename Pair<T>::raw*>(gr + goff);
-                if constexpr (KT == 4) c.q[j] = *reinterpret_cast<const uint32_t*>(qr + qoff);
-                else c.q[j] = *reinterpret_cast<const uint16_t*>(qr + qoff);
-                gr += p.ldg * (int64_t)sizeof(T);
-                qr += p.ldc;
-            }
-        } else {   // the range's end; one column
-#pragma unroll 1
-            for (int j = 0; j < 8; ++j) {
-                const int64_t m = base + j < m1 ? base + j : m1 - 1;
-                const char* gr = reinterpret_cast<const char*>(g + m * p.ldg);
-                const uint8_t* qr = p.codes + m * p.ldc;
-                typename Pair<T>::raw gv;
-                if (p.N > 1) gv = *reinterpret_cast<const typename Pair<T>::raw*>(gr + goff);
-                else gv = Pair<T>::one(reinterpret_cast<const T*>(gr));
-                uint32_t qv;
-                if constexpr (KT == 4) qv = *reinterpret_cast<const uint32_t*>(qr + qoff);
-                else qv = *reinterpret_cast<const uint16_t*>(qr + qoff);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {   // (no register is indexed by a variable)
-                    if (i == j) c.g[i] = gv, c.q[i] = qv;
-                }
-            }
+        for (int j = 0; j < 8; ++j) {
+            c.g[j] = *reinterpret_cast<const typename Pair<T>::raw*>(gr + goff);
+            if constexpr (KT == 4) c.q[j] = *reinterpret_cast<const uint32_t*>(qr + qoff);
+            else c.q[j] = *reinterpret_cast<const uint16_t*>(qr + qoff);
+            gr += p.ldg * (int64_t)sizeof(T);
+            qr += p.ldc;
         }
-        const int64_t group = (base < m1 ? base : m1 - 1) >> 3;   // base is a multiple of 8
-        c.s = *reinterpret_cast<const uint2*>(p.scales + group * p.lds + (kc >> 5) * 8);
+        c.s = *reinterpret_cast<const uint2*>(p.scales + (m >> 3) * p.lds + (kc >> 5) * 8);   // m is a multiple of 8
         if constexpr (NORM) {
-            const int64_t m = base + (lane & 7) < m1 ? base + (lane & 7) : m1 - 1;
-            c.r = p.rstd[m];
-            c.mu = p.mean[m];
+            c.r = p.rstd[m + (lane & 7)];
+            c.mu = p.mean[m + (lane & 7)];
         }
     };
-    auto place = [&](int chunk, const Chunk& c, uint4 (&A)[NC][4][TN], uint4 (&B)[4][TK]) {
-        const int64_t base = m0 + (int64_t)chunk * TM + 8 * wave;
-        const int rows = m1 - base < 8 ? (int)(m1 - base) : 8;   // rows from the range's end on count nothing
+    // the same at the range's end (rows from m1 on repeat the last one: place() drops them) and for a single column
+    auto fetch_end = [&](int64_t m, Chunk& c) {
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+            const int64_t mm = m + j < m1 ? m + j : m1 - 1;
+            const char* gr = reinterpret_cast<const char*>(g + mm * p.ldg);
+            const uint8_t* qr = p.codes + mm * p.ldc;
+            typename Pair<T>::raw gv;
+            if (p.N > 1) gv = *reinterpret_cast<const typename Pair<T>::raw*>(gr + goff);
+            else gv = Pair<T>::one(reinterpret_cast<const T*>(gr));
+            uint32_t qv;
+            if constexpr (KT == 4) qv = *reinterpret_cast<const uint32_t*>(qr + qoff);
+            else qv = *reinterpret_cast<const uint16_t*>(qr + qoff);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {   // (no register is indexed by a variable)
+                if (i == j) c.g[i] = gv, c.q[i] = qv;
+            }
+        }
+        c.s = *reinterpret_cast<const uint2*>(p.scales + ((m < m1 ? m : m1 - 1) >> 3) * p.lds + (kc >> 5) * 8);
+        if constexpr (NORM) {
+            const int64_t mm = m + (lane & 7) < m1 ? m + (lane & 7) : m1 - 1;
+            c.r = p.rstd[mm];
+            c.mu = p.mean[mm];
+        }
+    };
+    // a chunk's 8 rows as operand pieces; rows >= `rows` count nothing (their scale bytes need not be written)
+    auto place = [&](const Chunk& c, uint4 (&A)[NC][4][TN], uint4 (&B)[4][TK], auto with_sums, auto at_end, int rows) {
+        constexpr bool SUMS = decltype(with_sums)::value, ENDING = decltype(at_end)::value;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = Pair<T>::get(c.g[j], i);
-            if (rows < 8) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = j < rows ? v[j] : 0.f;
-            }
-            if (sums) sum[i] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-            if constexpr (NORM) {
-                float t = 0.f;
+            uint4 w[NC];
+            if constexpr (std::is_same<T, __bf16>::value && !NORM && !SUMS && !ENDING) {   // the values are their own only component
+                const uint32_t sel = i ? 0x07060302u : 0x05040100u;
+                w[0] = make_uint4(__builtin_amdgcn_perm(c.g[1].w[0], c.g[0].w[0], sel), __builtin_amdgcn_perm(c.g[3].w[0], c.g[2].w[0], sel),
+                                  __builtin_amdgcn_perm(c.g[5].w[0], c.g[4].w[0], sel), __builtin_amdgcn_perm(c.g[7].w[0], c.g[6].w[0], sel));
+            } else {
+                float v[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float r = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c.r), j));
-                    const float mu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c.mu), j));
-                    v[j] *= r;
-                    t = fmaf(v[j], mu, t);
+                    v[j] = Pair<T>::get(c.g[j], i);
+                    if constexpr (ENDING) v[j] = j < rows ? v[j] : 0.f;
                 }
-                muc[i] += t;
+                if constexpr (SUMS) sum[i] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                if constexpr (NORM) {
+                    float t = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float r = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c.r), j));
+                        const float mu = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(c.mu), j));
+                        v[j] *= r;
+                        t = fmaf(v[j], mu, t);
+                    }
+                    muc[i] += t;
+                }
+                split8<NC>(v, w);
             }
-            uint4 w[NC];
-            split8<NC>(v, w);
 #pragma unroll
             for (int k = 0; k < NC; ++k) A[k][wave][64 * i + lane] = w[k];
         }
@@ -280,12 +288,10 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
             const float s = act8_scale(((j < 4 ? c.s.x : c.s.y) >> (8 * (j & 3))) & 0xffu);
             e[j][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.q[j], s, false));
             if constexpr (KT == 4) e[j][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c.q[j], s, true));
-        }
-        if (rows < 8) {   // (scale bytes behind the last row are not written)
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
+            if constexpr (ENDING) {
 #pragma unroll
                 for (int h = 0; h < KT / 2; ++h) e[j][h] = j < rows ? e[j][h] : 0u;
+            }
         }
 #pragma unroll
         for (int h = 0; h < KT / 2; ++h) {
@@ -324,22 +330,48 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
         }
     };
 
-    // chunks in pairs, one per stage: a chunk behind the range's end is placed as zeros
-    fetch(0, R0);
-    fetch(1, R1);
-    place(0, R0, sA0, sB0);
-    fetch(2, R0);
-    __syncthreads();
-    for (int c = 0; c < chunks; c += 2) {
-        place(c + 1, R1, sA1, sB1);
-        fetch(c + 3, R1);
+    // whole pairs of chunks: no branch between the two barriers, so products and the next chunk's conversion interleave
+    const std::integral_constant<bool, true> yes{};
+    const std::integral_constant<bool, false> no{};
+    const int pairs = p.N > 1 ? (int)((m1 - m0) / (2 * TM)) : 0;
+    const int64_t mw = m0 + 8 * wave;
+    auto run = [&](auto with_sums) {
+        Chunk R;
+        const int last = 2 * pairs - 1;
+        auto at = [&](int chunk) { return mw + (int64_t)(chunk < last ? chunk : last) * TM; };
+        fetch(at(0), R);
+        place(R, sA0, sB0, with_sums, no, 8);
+        fetch(at(1), R);
+        __syncthreads();
+        for (int c = 0; c + 2 < 2 * pairs; c += 2) {
+            place(R, sA1, sB1, with_sums, no, 8);
+            fetch(at(c + 2), R);
+            multiply(sA0, sB0);
+            __syncthreads();
+            place(R, sA0, sB0, with_sums, no, 8);
+            fetch(at(c + 3), R);
+            multiply(sA1, sB1);
+            __syncthreads();
+        }
+        place(R, sA1, sB1, with_sums, no, 8);
         multiply(sA0, sB0);
         __syncthreads();
-        place(c + 2, R0, sA0, sB0);
-        fetch(c + 4, R0);
         multiply(sA1, sB1);
-        __syncthreads();
+    };
+    if (pairs > 0) {
+        if (sums) run(yes);
+        else run(no);
     }
+    for (int64_t m = m0 + (int64_t)pairs * 2 * TM; m < m1; m += TM) {   // what is left of the range
+        Chunk R;
+        fetch_end(m + 8 * wave, R);
+        __syncthreads();
+        const int64_t left = m1 - m - 8 * wave;
+        place(R, sA0, sB0, yes, yes, left < 8 ? (int)left : 8);
+        __syncthreads();
+        multiply(sA0, sB0);
+    }
+    __syncthreads();
 
     float (*sSum)[4][TN] = reinterpret_cast<float (*)[4][TN]>(&sA0[0][0][0]);   // column sums, behind the last product
     if (sums) {

@@ -486,26 +486,33 @@ ACTIVATION_CHECKPOINTS = (None, "e4m3")
 LAYER_NORM_MAX_WIDTH = 16384
 
 
-def _one_device(*tensors):
-    """every tensor on the same ROCm device -> that device"""
-    require_device(*tensors)
-    devs = {t.device for t in tensors if t is not None}
-    if len(devs) != 1:
-        raise RuntimeError(f"tensors on different devices: {sorted(str(d) for d in devs)}")
-    return devs.pop()
+def _one_device(first, *rest):
+    """every tensor on the same ROCm device -> its index (these calls are short: an index costs a tenth of a torch.device)"""
+    dev = first.get_device()
+    if dev < 0:
+        require_device(first)
+    for t in rest:
+        if t is not None and t.get_device() != dev:
+            require_device(t)
+            raise RuntimeError(f"tensors on different devices: {first.device} and {t.device}")
+    return dev
 
 
 class _device_guard:
-    """launches inside go to `dev`'s current stream, whatever device is current outside"""
+    """launches inside go to device `dev`'s current stream (`as` gives it), whatever device is current outside"""
+
+    __slots__ = ("dev", "prev")
 
     def __init__(self, dev):
         self.dev = dev
 
     def __enter__(self):
+        prev = torch.cuda.current_device()
         self.prev = None
-        if self.dev.index is not None and self.dev.index != torch.cuda.current_device():
-            self.prev = torch.cuda.current_device()
-            torch.cuda.set_device(self.dev.index)
+        if prev != self.dev:
+            self.prev = prev
+            torch.cuda.set_device(self.dev)
+        return torch._C._cuda_getCurrentRawStream(self.dev)
 
     def __exit__(self, *exc):
         if self.prev is not None:
@@ -513,14 +520,21 @@ class _device_guard:
         return False
 
 
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def _row_type(t):
-    if t.dtype not in ROW_TYPES:
+    k = ROW_TYPES.get(t.dtype)
+    if k is None:
         raise TypeError(f"expected float32, bfloat16 or float16, got {t.dtype}")
-    return ROW_TYPES[t.dtype]
+    return k
 
 
 def _rows(t):
     """[..., D] as a 2-D view with contiguous, non-overlapping rows (copied only if the layout forces it)"""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     if t.dim() < 1:
         raise ValueError("expected [..., D], got a scalar")
     if t.dim() != 2:
@@ -536,15 +550,18 @@ def _vector(t, n, what):
         return None
     if t.dtype != F32:
         raise TypeError(f"{what}: expected float32, got {t.dtype}")
-    if tuple(t.shape) != (n,):
+    if t.dim() != 1 or t.shape[0] != n:
         raise RuntimeError(f"{what}: expected shape ({n},), got {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _check_checkpoint(name):
     if name not in ACTIVATION_CHECKPOINTS:
         raise ValueError(f"activation checkpoint {name!r}: one of {ACTIVATION_CHECKPOINTS}")
     return name
+
+
+_NO_ACT8 = (None, 0, None, 0)
 
 
 class Act8:
@@ -575,9 +592,15 @@ class Act8:
 
     @classmethod
     def empty(cls, shape, dtype, device):
-        M, D = torch.Size(shape[:-1]).numel(), shape[-1]
-        return cls(torch.empty(M, cls.code_width(D), dtype=torch.uint8, device=device),
-                   torch.empty(-(-M // 8), cls.scale_width(D), dtype=torch.uint8, device=device), shape, dtype)
+        D = shape[-1]
+        if D < 1:
+            raise ValueError("Act8: width 0")
+        M = shape[0] if len(shape) == 2 else torch.Size(shape[:-1]).numel()
+        self = cls.__new__(cls)
+        self.codes = torch.empty(M, cls.code_width(D), dtype=torch.uint8, device=device)
+        self.scales = torch.empty(-(-M // 8), cls.scale_width(D), dtype=torch.uint8, device=device)
+        self.shape, self.dtype = shape, dtype
+        return self
 
     @property
     def device(self):
@@ -588,16 +611,15 @@ class Act8:
         return self.codes.numel() + self.scales.numel()
 
     def _args(self):   # the four arguments of the C ABI
-        return ptr(self.codes), self.codes.shape[1], ptr(self.scales), self.scales.shape[1]
+        return self.codes.data_ptr(), self.codes.shape[1], self.scales.data_ptr(), self.scales.shape[1]
 
     def unpack(self, dtype=None):
         """the values the codes stand for (rounded to `dtype`; default: the type that was packed)"""
         dtype = dtype or self.dtype
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
         t, M, D = _row_type(out), self.codes.shape[0], self.shape[-1]
-        _one_device(self.codes, self.scales)
-        with _device_guard(self.device):
-            check(lib().pcvae_act8_unpack(*self._args(), M, D, ptr(out), D, t, stream()), "act8_unpack")
+        with _device_guard(_one_device(self.codes, self.scales)) as st:
+            check(lib().pcvae_act8_unpack(*self._args(), M, D, out.data_ptr(), D, t, st), "act8_unpack")
         return out
 
 
@@ -606,9 +628,9 @@ def act8_pack(x):
     largest, the sign of "x > 0" exact"""
     dev = _one_device(x)
     t, rows = _row_type(x), _rows(x)
-    ck = Act8.empty(x.shape, x.dtype, dev)
-    with _device_guard(dev):
-        check(lib().pcvae_act8_pack(ptr(rows), _ld(rows), t, rows.shape[0], rows.shape[1], *ck._args(), stream()), "act8_pack")
+    ck = Act8.empty(x.shape, x.dtype, x.device)
+    with _device_guard(dev) as st:
+        check(lib().pcvae_act8_pack(rows.data_ptr(), _ld(rows), t, rows.shape[0], rows.shape[1], *ck._args(), st), "act8_pack")
     return ck
 
 
@@ -620,8 +642,8 @@ def act8_leaky_bwd_(g, ck):
     rows = _rows(g)
     if rows.data_ptr() != g.data_ptr():
         raise ValueError("act8_leaky_bwd: works in place on rows with unit column stride")
-    with _device_guard(dev):
-        check(lib().pcvae_act8_leaky_bwd(ptr(rows), _ld(rows), _row_type(g), *ck._args(), rows.shape[0], rows.shape[1], stream()),
+    with _device_guard(dev) as st:
+        check(lib().pcvae_act8_leaky_bwd(rows.data_ptr(), _ld(rows), _row_type(g), *ck._args(), rows.shape[0], rows.shape[1], st),
               "act8_leaky_bwd")
     return g
 
@@ -652,12 +674,13 @@ def act8_bwd_weight_raw(gy, ck, dW=None, db=None, norm=None):
             raise RuntimeError(f"act8_bwd_weight: dW ({N}, {K}) with contiguous rows and contiguous db ({N},) expected, got "
                                f"{tuple(dW.shape)} / {tuple(db.shape)}")
     else:
-        dW, db = torch.empty(N, K, dtype=F32, device=dev), torch.empty(N, dtype=F32, device=dev)
-    with _device_guard(dev):
-        nbytes = lib().pcvae_act8_bwd_weight_ws_bytes(M, N, K)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check(lib().pcvae_act8_bwd_weight(ptr(rows), _ld(rows), t, *ck._args(), M, N, K, ptr(mean), ptr(rstd), ptr(w), ptr(b), ptr(dW),
-                                          _ld(dW), ptr(db), int(accumulate), ptr(ws), nbytes, stream()), "act8_bwd_weight")
+        dW, db = gy.new_empty(N, K, dtype=F32), gy.new_empty(N, dtype=F32)
+    L = lib()
+    with _device_guard(dev) as st:
+        nbytes = L.pcvae_act8_bwd_weight_ws_bytes(M, N, K)
+        ws = gy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        check(L.pcvae_act8_bwd_weight(rows.data_ptr(), _ld(rows), t, *ck._args(), M, N, K, _at(mean), _at(rstd), _at(w), _at(b),
+                                      dW.data_ptr(), _ld(dW), db.data_ptr(), accumulate, _at(ws), nbytes, st), "act8_bwd_weight")
     return dW, db
 
 
@@ -669,12 +692,11 @@ def layer_norm_fwd_raw(x, weight=None, bias=None, eps=1e-5, checkpoint=None):
     t, rows = _row_type(x), _rows(x)
     M, D = rows.shape
     weight, bias = _vector(weight, D, "layer_norm: weight"), _vector(bias, D, "layer_norm: bias")
-    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    mean, rstd = torch.empty(M, dtype=F32, device=dev), torch.empty(M, dtype=F32, device=dev)
-    ck = Act8.empty(x.shape, x.dtype, dev) if checkpoint else None
-    with _device_guard(dev):
-        check(lib().pcvae_layer_norm_fwd(ptr(rows), _ld(rows), t, M, D, ptr(weight), ptr(bias), float(eps), ptr(y), D, ptr(mean),
-                                         ptr(rstd), *(ck._args() if ck else (None, 0, None, 0)), stream()), "layer_norm_fwd")
+    y, mean, rstd = x.new_empty(x.shape), x.new_empty(M, dtype=F32), x.new_empty(M, dtype=F32)
+    ck = Act8.empty(x.shape, x.dtype, x.device) if checkpoint else None
+    with _device_guard(dev) as st:
+        check(lib().pcvae_layer_norm_fwd(rows.data_ptr(), _ld(rows), t, M, D, _at(weight), _at(bias), eps, y.data_ptr(), D, mean.data_ptr(),
+                                         rstd.data_ptr(), *(ck._args() if ck else _NO_ACT8), st), "layer_norm_fwd")
     return y, mean, rstd, ck
 
 
@@ -682,8 +704,7 @@ def layer_norm_bwd_raw(gy, x, weight, mean, rstd, dweight=None, dbias=None, leak
     """-> (dx, dweight, dbias) of layer_norm at x (a tensor of gy's type, or the Act8 the forward kept).  leaky: x is a LeakyReLU's
     output and dx is taken through it, to its input.  Given dweight / dbias buffers are accumulated into; None: new ones."""
     kept = isinstance(x, Act8)
-    parts = (x.codes, x.scales) if kept else (x,)
-    dev = _one_device(gy, *parts, weight, mean, rstd, dweight, dbias)
+    dev = _one_device(gy, x.codes if kept else x, x.scales if kept else None, weight, mean, rstd, dweight, dbias)
     if gy.shape != x.shape:
         raise RuntimeError(f"layer_norm: gradient {tuple(gy.shape)} of rows {tuple(x.shape)}")
     if not kept and gy.dtype != x.dtype:
@@ -703,15 +724,16 @@ def layer_norm_bwd_raw(gy, x, weight, mean, rstd, dweight=None, dbias=None, leak
             if not b.is_contiguous():
                 raise ValueError("layer_norm: gradient buffers are contiguous")
     else:
-        dweight, dbias = torch.empty(D, dtype=F32, device=dev), torch.empty(D, dtype=F32, device=dev)
+        dweight, dbias = gy.new_empty(D, dtype=F32), gy.new_empty(D, dtype=F32)
     rows = None if kept else _rows(x)
-    dx = torch.empty(gy.shape, dtype=gy.dtype, device=dev)
-    with _device_guard(dev):
-        nbytes = lib().pcvae_layer_norm_bwd_ws_bytes(M, D, t)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        check(lib().pcvae_layer_norm_bwd(ptr(g), _ld(g), t, M, D, ptr(rows), 0 if kept else _ld(rows),
-                                         *(x._args() if kept else (None, 0, None, 0)), ptr(weight), ptr(mean), ptr(rstd), int(bool(leaky)),
-                                         ptr(dx), D, ptr(dweight), ptr(dbias), int(accumulate), ptr(ws), nbytes, stream()),
+    dx = gy.new_empty(gy.shape)
+    L = lib()
+    with _device_guard(dev) as st:
+        nbytes = L.pcvae_layer_norm_bwd_ws_bytes(M, D, t)
+        ws = gy.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        check(L.pcvae_layer_norm_bwd(g.data_ptr(), _ld(g), t, M, D, _at(rows), 0 if kept else _ld(rows),
+                                     *(x._args() if kept else _NO_ACT8), _at(weight), mean.data_ptr(), rstd.data_ptr(), bool(leaky),
+                                     dx.data_ptr(), D, dweight.data_ptr(), dbias.data_ptr(), accumulate, _at(ws), nbytes, st),
               "layer_norm_bwd")
     return dx, dweight, dbias
 
