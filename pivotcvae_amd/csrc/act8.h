@@ -191,10 +191,6 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 
 // ---- 8-bit blocks -----------------------------------------------------------------------------------------------------------------
 constexpr uint32_t kAct8Cap = 0x7f700000u;   // 1.875 * 2^127
-__device__ __forceinline__ uint32_t act8_magnitude(float x) {   // |x|'s bits as the block maximum counts them
-    const uint32_t a = __float_as_uint(x) & 0x7fffffffu;
-    return a >= 0x7f800000u ? 0u : (a < kAct8Cap ? a : kAct8Cap);
-}
 __device__ __forceinline__ uint32_t act8_byte(uint32_t top) {
     const uint32_t e = (top + 0x1fffffu) >> 23;
     return e > 18u ? e - 8u : 10u;
@@ -202,34 +198,34 @@ __device__ __forceinline__ uint32_t act8_byte(uint32_t top) {
 __device__ __forceinline__ float act8_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 __device__ __forceinline__ float act8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-// four values -> four codes (the lowest byte is the first)
-__device__ __forceinline__ uint32_t act8_codes(const float* x, float inv) {
+// four values -> four codes (the lowest byte is the first).  Any values:
+__device__ __forceinline__ uint32_t act8_codes_any(const float* x, float inv) {
+    const float cap = __uint_as_float(kAct8Cap);
     float v[4];
-    bool bad = false;
+    uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float cap = __uint_as_float(kAct8Cap);
-        bad |= (__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u;
+        if ((__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u) bad |= 0x7fu << (8 * i);
         v[i] = fminf(fmaxf(x[i], -cap), cap) * inv;
         v[i] = v[i] > 0.f ? fmaxf(v[i], 0x1p-9f) : v[i];
     }
     int r = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
     r = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], r, true);
-    uint32_t codes = (uint32_t)r;
-    if (bad) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f800000u) codes |= 0x7fu << (8 * i);
-    }
-    return codes;
+    return (uint32_t)r | bad;
+}
+// ... all of them finite, at most the cap and at least 2^-9 of the scale: the conversion alone
+__device__ __forceinline__ uint32_t act8_codes_plain(const float* x, float inv) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, r, true);
+    return (uint32_t)r;
 }
 // four codes -> their values
 __device__ __forceinline__ void act8_values(uint32_t codes, float scale, float* v) {
-    const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-    v[0] = a[0] * scale;
-    v[1] = a[1] * scale;
-    v[2] = b[0] * scale;
-    v[3] = b[1] * scale;
+    const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, false), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(codes, scale, true);
+    v[0] = a[0];
+    v[1] = a[1];
+    v[2] = b[0];
+    v[3] = b[1];
 }
 
 // where a block's scale byte lies: 8 rows side by side ([ceil(M / 8)][blocks][8 rows], ld bytes per 8 rows), so that the weight gradient's
@@ -243,24 +239,44 @@ __device__ __forceinline__ B* act8_scale_at(B* scales, int64_t ld, int64_t row, 
 // Every lane of the block takes part, whatever its columns (values from D on are zeros); columns from D on get code 0.
 template <int VW>
 __device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, uint8_t* codes, uint8_t* scale) {
-    uint32_t top = 0;
+    // magnitudes as integers: NaN and infinity are the largest.  3.5 vector operations per value unless a lane of the wave holds a bad, a
+    // huge or a tiny (zero) value; then the block's maximum is taken again over the finite ones.
+    uint32_t top = 0, low = 0xffffffffu;
 #pragma unroll
     for (int i = 0; i < VW; ++i) {
-        const uint32_t m = act8_magnitude(v[i]);
-        top = m > top ? m : top;
+        const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+        top = a > top ? a : top;
+        low = a < low ? a : low;
     }
     top = lanes_max<kAct8Block / VW>(top);
+    const bool odd = top > kAct8Cap;   // (uniform over the block's lanes)
+    if (odd) {
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < VW; ++i) {
+            uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+            a = a >= 0x7f800000u ? 0u : (a < kAct8Cap ? a : kAct8Cap);
+            top = a > top ? a : top;
+        }
+        top = lanes_max<kAct8Block / VW>(top);
+    }
     const uint32_t byte = act8_byte(top);
     const float inv = act8_inverse(byte);
+    uint32_t w[VW / 4];
+    if (odd || low < (byte - 9u) << 23) {
+#pragma unroll
+        for (int h = 0; h < VW / 4; ++h) w[h] = act8_codes_any(v + 4 * h, inv);
+    } else {
+#pragma unroll
+        for (int h = 0; h < VW / 4; ++h) w[h] = act8_codes_plain(v + 4 * h, inv);
+    }
     if (c < Dp) {
-        if constexpr (VW == 4) {
-            *reinterpret_cast<uint32_t*>(codes + c) = act8_codes(v, inv);
-        } else {
-            *reinterpret_cast<uint2*>(codes + c) = make_uint2(act8_codes(v, inv), act8_codes(v + 4, inv));
-        }
+        if constexpr (VW == 4) *reinterpret_cast<uint32_t*>(codes + c) = w[0];
+        else *reinterpret_cast<uint2*>(codes + c) = make_uint2(w[0], w[1]);
         if ((c & (kAct8Block - 1)) == 0) *scale = (uint8_t)byte;
     }
 }
+
 // host: the types of a row
 static inline int row_type_size(int t) { return t == PCVAE_ROW_F32 ? 4 : 2; }
 // codes [M, ldc >= ceil(D / 32) * 32] at a multiple of 16 bytes, scale bytes [ceil(M / 8), lds >= 8 ceil(D / 32)] at a

@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void act8_rows_kernel(RowsParams p) {
     }
 }
 
-constexpr int kRowsGroups = 4096;
+constexpr int kRowsGroups = 8192;   // 32 waves per CU of the launch's stride (2048 .. 16384 measured: 54.7, 53.4, 51.7, 51.6 us on 8192 x 5397)
 
 template <int WHAT>
 int launch_rows(const char* what, int type, const RowsParams& p0, pcvae_stream_t stream) {
@@ -336,24 +336,27 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
     const int pairs = p.N > 1 ? (int)((m1 - m0) / (2 * TM)) : 0;
     const int64_t mw = m0 + 8 * wave;
     auto run = [&](auto with_sums) {
-        Chunk R;
+        constexpr int AHEAD = KT == 2 ? 2 : 1;   // chunks in flight: the wide tile's accumulators leave registers for one
+        Chunk R0, R1v;
+        Chunk& R1 = AHEAD == 2 ? R1v : R0;
         const int last = 2 * pairs - 1;
         auto at = [&](int chunk) { return mw + (int64_t)(chunk < last ? chunk : last) * TM; };
-        fetch(at(0), R);
-        place(R, sA0, sB0, with_sums, no, 8);
-        fetch(at(1), R);
+        fetch(at(0), R0);
+        if (AHEAD == 2) fetch(at(1), R1);
+        place(R0, sA0, sB0, with_sums, no, 8);
+        fetch(at(AHEAD), R0);
         __syncthreads();
         for (int c = 0; c + 2 < 2 * pairs; c += 2) {
-            place(R, sA1, sB1, with_sums, no, 8);
-            fetch(at(c + 2), R);
+            place(R1, sA1, sB1, with_sums, no, 8);
+            fetch(at(c + 1 + AHEAD), R1);
             multiply(sA0, sB0);
             __syncthreads();
-            place(R, sA0, sB0, with_sums, no, 8);
-            fetch(at(c + 3), R);
+            place(R0, sA0, sB0, with_sums, no, 8);
+            fetch(at(c + 2 + AHEAD), R0);
             multiply(sA1, sB1);
             __syncthreads();
         }
-        place(R, sA1, sB1, with_sums, no, 8);
+        place(R1, sA1, sB1, with_sums, no, 8);
         multiply(sA0, sB0);
         __syncthreads();
         multiply(sA1, sB1);
@@ -436,11 +439,36 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
 template <int SL>
 __global__ __launch_bounds__(256) void act8_weight_join_kernel(DwParams p, int TK) {
     __shared__ f32x4_t sh[256];
+    const int sum_groups = p.db ? (p.N + 31) / 32 : 0;
+    if ((int)blockIdx.x < sum_groups) {   // 32 column sums, 8 runs of ranges each
+        float* part = reinterpret_cast<float*>(sh);
+        const int n = blockIdx.x * 32 + (threadIdx.x & 31), run = threadIdx.x >> 5, per = (p.nz + 7) / 8;
+        const int z0 = run * per, z1 = z0 + per < p.nz ? z0 + per : p.nz;
+        float s = 0.f;
+        if (n < p.N) {
+            for (int z = z0; z < z1; z += 8) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = z + j < z1 ? p.part_db[(int64_t)(z + j) * p.nn * TN + n] : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s += v[j];
+            }
+        }
+        part[threadIdx.x] = s;
+        __syncthreads();
+        if (run == 0 && n < p.N) {
+#pragma unroll
+            for (int r = 1; r < 8; ++r) s += part[r * 32 + threadIdx.x];
+            p.db[n] = p.accumulate ? p.db[n] + s : s;
+        }
+        return;
+    }
+    const int block = blockIdx.x - sum_groups, blocks = gridDim.x - sum_groups;
     const int tiles = p.nn * p.nk, per_tile = TN * TK / 4, cols = 256 / SL;
     const int64_t total = (int64_t)tiles * per_tile;
     const int slice = threadIdx.x / cols, at = threadIdx.x % cols;
     const int per = (p.nz + SL - 1) / SL, z0 = slice * per, z1 = z0 + per < p.nz ? z0 + per : p.nz;
-    for (int64_t i0 = (int64_t)blockIdx.x * cols; i0 < total; i0 += (int64_t)gridDim.x * cols) {   // total is a multiple of cols
+    for (int64_t i0 = (int64_t)block * cols; i0 < total; i0 += (int64_t)blocks * cols) {   // total is a multiple of cols
         const int64_t i = i0 + at;
         const int tile = (int)(i / per_tile), e = (int)(i % per_tile) * 4;
         const int n = tile / p.nk * TN + e / TK, k = tile % p.nk * TK + e % TK;
@@ -474,13 +502,6 @@ __global__ __launch_bounds__(256) void act8_weight_join_kernel(DwParams p, int T
                 if (k + j < p.K) out[j] = p.accumulate ? out[j] + s[j] : s[j];
         }
     }
-    if (p.db) {
-        for (int64_t n = (int64_t)blockIdx.x * 256 + threadIdx.x; n < p.N; n += (int64_t)gridDim.x * 256) {
-            float s = 0.f;
-            for (int z = 0; z < p.nz; ++z) s += p.part_db[(int64_t)z * p.nn * TN + n];
-            p.db[n] = p.accumulate ? p.db[n] + s : s;
-        }
-    }
 }
 
 __global__ __launch_bounds__(256) void act8_weight_empty_kernel(DwParams p) {
@@ -491,14 +512,19 @@ __global__ __launch_bounds__(256) void act8_weight_empty_kernel(DwParams p) {
     }
 }
 
-// tile width and ranges of rows
+// Tile width and ranges of rows.  The wide tile (128 x 256) converts less per product, the narrow one (128 x 128) has two chunks in flight
+// and half the partial tile per range: measured on 8192 rows, us of 128 / 256 columns: 256 x 256 24 / 27, 256 x 1419 43 / 42, 1152 x 256
+// 38 / 37; on 16384 rows 1024 x 2048 245 / 212; 32768 rows 4864 x 1024 1120 / 905.  It is taken from 2048 chunks of 32 rows on, over all tiles.
+// Ranges: the fewest rounds of 512 resident workgroups, a chunk's time against the partial tiles' traffic (flat: within 5 % over a factor
+// of two in the number of ranges).
 struct DwPlan { int kt, nn, nk, nz; int64_t m_per; };
 DwPlan dw_plan(int64_t M, int64_t N, int64_t K) {
     DwPlan d;
-    d.kt = K > 128 ? 4 : 2;
+    const int64_t chunks = cdiv(M, TM);
+    d.kt = K > 128 && cdiv(N, TN) * cdiv(K, 256) * chunks >= 2048 ? 4 : 2;
     d.nn = (int)cdiv(N, TN);
     d.nk = (int)cdiv(K, 64 * d.kt);
-    const int64_t tiles = (int64_t)d.nn * d.nk, chunks = cdiv(M, TM);
+    const int64_t tiles = (int64_t)d.nn * d.nk;
     double best = 0.;
     int64_t pick = 1;
     for (int64_t nz = 1; nz <= 64 && nz * 2 <= chunks + 1; ++nz) {
@@ -529,13 +555,12 @@ int launch_dw(const DwParams& p, int kt, pcvae_stream_t stream) {
     if (int rc = check_launch("act8_bwd_weight")) return rc;
     if (p.nz == 1) return PCVAE_OK;
     const int64_t vecs = (int64_t)p.nn * p.nk * TN * 64 * kt / 4;
-    if (p.nz >= 8) {
-        const int64_t groups = cdiv(vecs, 32);
-        hipLaunchKernelGGL(act8_weight_join_kernel<8>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, as_stream(stream), p, 64 * kt);
-    } else {
-        const int64_t groups = cdiv(vecs, 256);
-        hipLaunchKernelGGL(act8_weight_join_kernel<1>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, as_stream(stream), p, 64 * kt);
-    }
+    const int64_t sums = p.db ? cdiv(p.N, 32) : 0;
+    auto grid_of = [&](int cols) { return dim3((unsigned)(sums + (cdiv(vecs, cols) < 4096 ? cdiv(vecs, cols) : 4096))); };
+    if (p.nz >= 8)
+        hipLaunchKernelGGL(act8_weight_join_kernel<8>, grid_of(32), dim3(256), 0, as_stream(stream), p, 64 * kt);
+    else
+        hipLaunchKernelGGL(act8_weight_join_kernel<1>, grid_of(256), dim3(256), 0, as_stream(stream), p, 64 * kt);
     return check_launch("act8_bwd_weight (join)");
 }
 

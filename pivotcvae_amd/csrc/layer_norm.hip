@@ -18,7 +18,6 @@ using namespace pcvae;
 namespace {
 
 constexpr int kMaxWidth = 16384;
-constexpr int kBwdGroups = 512;   // workgroups of a backward launch at most: two per CU, and so many partial rows to join
 
 struct FwdParams {
     const void* x; int64_t ldx;
@@ -348,9 +347,16 @@ int with_type(int t, F f) {
 
 int vector_width(int t) { return t == PCVAE_ROW_F32 ? 4 : 8; }
 int rows_per_group(const Plan& pl) { return pl.tpr >= 256 ? 1 : 256 / pl.tpr; }
+// Workgroups of a launch at most.  A forward's loads its parameters once per workgroup (1024 / 4096, measured on 8192 x 5397 fp32: 76 / 81 us
+// with 1024 threads per row, on 32768 x 2048 bf16: 62 / 58 us with 256); each of a backward's leaves a partial row of column sums (256 / 512 /
+// 768: 8192 x 5397 fp32 108 / 116 / 124 us, 32768 x 2048 bf16 118 / 84 / 83 us, 65536 x 256 fp32 from codes 60 / 40 / 36 us)
+int fwd_groups(int64_t M, const Plan& pl) {
+    const int64_t n = cdiv(M, rows_per_group(pl)), most = pl.tpr == 1024 ? 1024 : 4096;
+    return (int)(n < most ? n : most);
+}
 int bwd_groups(int64_t M, const Plan& pl) {
-    const int64_t n = cdiv(M, rows_per_group(pl));
-    return (int)(n < kBwdGroups ? n : kBwdGroups);
+    const int64_t n = cdiv(M, rows_per_group(pl)), most = pl.tpr == 1024 ? 256 : (pl.tpr <= 64 && pl.nv == 1 ? 768 : 512);
+    return (int)(n < most ? n : most);
 }
 
 int check_rows(const char* who, int type, int64_t M, int D, int64_t ld, const void* p) {
@@ -377,8 +383,7 @@ extern "C" int pcvae_layer_norm_fwd(const void* x, int64_t ldx, int type, int64_
     if (M == 0) return PCVAE_OK;
     const Plan pl = plan(D, vector_width(type));
     FwdParams p{x, ldx, weight, bias, y, ldy, mean, rstd, codes, ldc, scales, lds, M, D, (int)cdiv(D, kAct8Block) * kAct8Block, eps};
-    const int64_t groups = cdiv(M, rows_per_group(pl));
-    const unsigned grid = (unsigned)(groups < 2048 ? groups : 2048);
+    const unsigned grid = (unsigned)fwd_groups(M, pl);
     return with_type(type, [&](auto* tag) {
         using T = std::remove_pointer_t<decltype(tag)>;
         return with_plan<RowType<T>::VW>(pl, [&](auto t, auto n, auto e) {
