@@ -328,6 +328,24 @@ def test_weight_gradient_bad_values_stay_in_their_row_and_column():
     assert bool(db[9].isnan()) and int(db.isnan().sum()) == 1
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,N,K,normed", [(8197, 300, 520, False), (8200, 301, 519, True), (16421, 129, 1000, False)])
+def test_weight_gradient_in_wide_tiles(M, N, K, normed, t):
+    """over 2048 chunks of 32 rows in all tiles: 128 x 256 tiles, several ranges of rows and a ragged last one"""
+    assert -(-N // 128) * -(-K // 256) * -(-M // 32) >= 2048
+    x, g = rand((M, K), 11, torch.float32, 2.0).to(DEV), rand((M, N), 12, t, 0.1, leaky=False).to(DEV)
+    ck = ops().act8_pack(x)
+    norm = None
+    if normed:
+        _, mean, rstd, _ = ops().layer_norm_fwd_raw(x)
+        norm = (mean, rstd, *(p.to(DEV) for p in params(K, K)))
+    dW, db = ops().act8_bwd_weight_raw(g, ck, norm=norm)
+    want, bound, wdb, bdb = weight_grad(g, kept64(x), norm)
+    inside(dW, want, bound, "dW")
+    inside(db, wdb, bdb, "db")
+    assert torch.equal(ops().act8_bwd_weight_raw(g, ck, norm=norm)[0], dW)
+
+
 def test_rows_behind_offsets_over_32_bits():
     """row strides that take a batch past 2^31 elements, and 2^32 bytes of codes"""
     ld, M, D = 1 << 20, 2100, 40
@@ -401,16 +419,13 @@ def _to(dev_pairs):
     return [tuple(t.to(DEV).requires_grad_() for t in p) for p in dev_pairs]
 
 
-@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
-@pytest.mark.parametrize("normed", [False, True])
+@pytest.mark.parametrize("normed,checkpoint", [(False, "e4m3"), (True, None), (True, "e4m3")])
 @pytest.mark.parametrize("shape", ["mlp linear", "mlp activated", "heads"])
 def test_stack_with_norms_and_checkpoints(shape, normed, checkpoint):
     """a stack's outputs and every gradient against a 64-bit pass that keeps what the stack keeps.  Activations are taken from the same
     forward kernels run layer by layer (their own bits decide the codes); gradients of a stack of three layers of width <= 60 over 75
     rows in fp32: every value passes at most 8 sums of 75 terms, so 1e-5 of the largest magnitude (160 u) is allowed"""
     o = ops()
-    if not normed and checkpoint is None:
-        pytest.skip("the plain stack: other tests")
     widths, M = [37, 60, 33, 20], 75
     layers, nrm = _stack(widths, 4, normed)
     heads = shape == "heads"
