@@ -624,7 +624,7 @@ class Act8:
 
 
 def act8_pack(x):
-    """x [..., D] (fp32 / bf16 / fp16) -> Act8: 1.03 bytes per value; relative error at most 2^-4 per value above 2^-14 of its block's
+    """x [..., D] (fp32 / bf16 / fp16) -> Act8: 1.03 bytes per value; relative error at most 2^-4 per value above 2^-13 of its block's
     largest, the sign of "x > 0" exact"""
     dev = _one_device(x)
     t, rows = _row_type(x), _rows(x)
