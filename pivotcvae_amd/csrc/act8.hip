@@ -6,9 +6,9 @@
 //            (h = (q - mu_m) r_m, the layer's input w_k h + b_k):  dW = w_k (sum_m (g r_m) q - sum_m g r_m mu_m) + b_k db
 //
 // Bounds.  The row kernels: memory (8192 x 5397 fp32 pack 50 us = 4.4 TB/s of codes and values, unpack 35-50 us; a device copy runs at
-// 4.95 TB/s).  The weight gradient: the matrix pipe - 4864 x 1024 over 32768 rows, fp32 g, 860 us = 380 TFLOP/s of fp32-exact products =
-// 1140 TFLOP/s of bf16 products issued, 0.93 of what the library's largest bf16 product reaches (1225) - and, for one component (bf16 g),
-// the instructions around its products: 2048 x 2048 over 16384 rows 165 us = 830 TFLOP/s (matrix pipe 0.36 busy, LDS 0.27, vector
+// 4.95 TB/s).  The weight gradient: the matrix pipe - 4864 x 1024 over 32768 rows, fp32 g, 850-920 us = 355-384 TFLOP/s of fp32-exact
+// products = 1065-1150 TFLOP/s of bf16 products issued, 0.87-0.94 of what the library's largest bf16 product reaches (1225) - and, for one
+// component (bf16 g), the instructions around its products: 2048 x 2048 over 16384 rows 172 us = 800 TFLOP/s (matrix pipe 0.36 busy, LDS 0.27, vector
 // issue 0.28: two waves per SIMD do not cover each other's waits).  Small ones are launches and latency: 256 x 256 over 8192 rows 24 us.
 #include "act8.h"
 

@@ -129,6 +129,46 @@ def test_layer_norm_without_parameters_and_accumulating():
     assert out[1] is dw0 and torch.equal(dw0, 2.0 + dw) and torch.equal(db0, -3.0 + db)
 
 
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("M,D", [(1, 40), (30, 5), (301, 256), (4099, 99), (700, 2048), (300, 5397)])
+def test_layer_norm_backward_over_its_own_gradient(M, D, t):
+    """the C entry point with dx in g's memory"""
+    from pivotcvae_amd import _hip
+    x, g = rand((M, D), 1, t).to(DEV), rand((M, D), 2, t, 0.1, leaky=False).to(DEV)
+    w, _ = (p.to(DEV) for p in params(D, 1))
+    _, mean, rstd, _ = ops().layer_norm_fwd_raw(x, w)
+    dx, dw, db = ops().layer_norm_bwd_raw(g, x, w, mean, rstd)
+    L, k = _hip.lib(), _hip.ROW_TYPES[t]
+    n = L.pcvae_layer_norm_bwd_ws_bytes(M, D, k)
+    ws, dw2, db2 = torch.empty(n, dtype=torch.uint8, device=DEV), torch.empty_like(dw), torch.empty_like(db)
+    _hip.check(L.pcvae_layer_norm_bwd(g.data_ptr(), D, k, M, D, x.data_ptr(), D, None, 0, None, 0, w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), 0,
+                                      g.data_ptr(), D, dw2.data_ptr(), db2.data_ptr(), 0, ws.data_ptr(), n, _hip.stream()))
+    assert torch.equal(g, dx) and torch.equal(dw2, dw) and torch.equal(db2, db)
+
+
+def test_refusals_on_the_device():
+    o = ops()
+    x = rand((6, 64), 1).to(DEV)
+    y, mean, rstd, ck = o.layer_norm_fwd_raw(x, checkpoint="e4m3")
+    for err, call in ((TypeError, lambda: o.layer_norm_fwd_raw(x.double())), (TypeError, lambda: o.layer_norm_fwd_raw(x, x[0].half())),
+                      (RuntimeError, lambda: o.layer_norm_fwd_raw(x, x[0, :5].contiguous())), (RuntimeError, lambda: o.layer_norm_fwd_raw(x, eps=-1.0)),
+                      (RuntimeError, lambda: o.layer_norm_fwd_raw(torch.zeros(2, 16385, device=DEV))), (RuntimeError, lambda: o.layer_norm_fwd_raw(x[:, :0])),
+                      (RuntimeError, lambda: o.layer_norm_fwd_raw(x, mean.cpu())), (RuntimeError, lambda: o.layer_norm_bwd_raw(x[:5], x, None, mean, rstd)),
+                      (TypeError, lambda: o.layer_norm_bwd_raw(x.half(), x, None, mean, rstd)), (ValueError, lambda: o.layer_norm_bwd_raw(x, x, None, None, rstd)),
+                      (RuntimeError, lambda: o.layer_norm_bwd_raw(x, x, None, mean[:3], rstd)), (ValueError, lambda: o.act8_pack(x[:, :0])),
+                      (ValueError, lambda: o.layer_norm_bwd_raw(x, x, None, mean, rstd, dweight=x[0])), (RuntimeError, lambda: o.act8_bwd_weight_raw(x[:5], ck)),
+                      (ValueError, lambda: o.act8_bwd_weight_raw(x, ck, dW=torch.zeros(64, 64, device=DEV))),
+                      (RuntimeError, lambda: o.act8_bwd_weight_raw(x, ck, torch.zeros(64, 63, device=DEV), torch.zeros(64, device=DEV))),
+                      (ValueError, lambda: o.act8_bwd_weight_raw(x, ck, norm=(mean, None, None, None))), (RuntimeError, lambda: o.act8_leaky_bwd_(x[:, :3], ck)),
+                      (ValueError, lambda: o.act8_leaky_bwd_(x.t().contiguous().t(), ck)), (TypeError, lambda: o.act8_bwd_weight_raw(x.double(), ck))):
+        with pytest.raises(err):
+            call()
+    a = x.clone().requires_grad_()
+    (ga,) = torch.autograd.grad(o.layer_norm(a).sum(), a, create_graph=True)
+    with pytest.raises(RuntimeError):   # second derivatives
+        ga.sum().backward()
+
+
 def test_layer_norm_of_constant_rows_bad_values_and_no_rows():
     x = rand((6, 96), 8).to(DEV)
     x[1] = 0.0
