@@ -424,6 +424,8 @@ int pcvae_relu_bwd(float* g, int64_t ldg, const float* y, int64_t ldy, int64_t r
  * Layer norm over the rows of x [M, D] (1 <= D <= 16384), forward and backward.  No counterpart in the reference (its stacks are
  * Linear + LeakyReLU only): for stacks with a norm between their layers.
  *     fwd : mean[m], rstd[m] = 1 / sqrt(var + eps) (both optional, fp32) ;  y = (x - mean) rstd weight + bias (NULL: 1 / 0)
+ *           (any finite row, whatever its magnitude, whose values lie less than fp32's largest number from their mean; a row
+ *           with NaN or +-inf: statistics and y NaN)
  *           codes / scales: optionally the 8-bit form of x (below), from the same pass
  *     bwd : h = (x - mean) rstd ;  dx = rstd (w g - mean(w g) - h mean(w g h)), times LeakyReLU'(x) with `leaky` (x is then a
  *           LeakyReLU's output) ;  dweight[c] = sum_m g h,  dbias[c] = sum_m g (either may be NULL; accumulate: added to what is there).

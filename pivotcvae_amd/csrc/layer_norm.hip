@@ -4,7 +4,8 @@
 //   dx = r (w g - mean(w g) - h mean(w g h))  [* LeakyReLU'(x): x a LeakyReLU's output],   dw = sum_m g h,   db = sum_m g
 //
 // Both directions read every operand once and keep the row in registers between the passes over it (the variance is taken about the
-// mean, not from a difference of moments); statistics and sums are fp32.  TPR neighbouring threads own a row, each holds NV pieces of
+// mean, not from a difference of moments; rows whose squares or sum leave fp32's range are taken at 2^-80 of their size, so every finite row
+// has its statistics, and a row that holds NaN or an infinity has NaN for both); statistics and sums are fp32.  TPR neighbouring threads own a row, each holds NV pieces of
 // 16 bytes of it (8 lanes to 16 waves; rule: plan()).  Any of the row types fp32 / bf16 / fp16, any width up to 16384, any row
 // stride.  The forward optionally also writes the row's 8-bit form (act8.h), and the backward takes x from it: the norm's saved input
 // is then one byte per value, and LeakyReLU' reads off its codes.
@@ -118,8 +119,34 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(F
         }
         // what the first sum's roundings left of the mean shows in the deviations' own mean: rows far from zero (and constant ones) need it
         row_sum<TPR, 2>(m, red1, 0);
-        const float rest = m[0] / p.D, mean = near + rest;
-        const float rstd = 1.f / sqrtf(fmaxf(m[1] / p.D - rest * rest, 0.f) + p.eps);
+        const float rest = m[0] / p.D;
+        float mean = near + rest, rstd = 1.f / sqrtf(fmaxf(m[1] / p.D - rest * rest, 0.f) + p.eps);
+        if (!(m[1] < INFINITY)) {   // (the same for every thread of a row; rows of more than a wave have their workgroup to themselves)
+            // Squares or the sum out of fp32's range: the statistics again, of the row times 2^-80 - its values are then below 2^48, the sums
+            // below 2^110, and what vanishes is under 2^-80 of the largest deviation.  A row that holds NaN or an infinity stays NaN.
+            float far[1] = {0.f}, dev[2] = {0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) far[0] = fmaf(v[k][i], 0x1p-80f, far[0]);
+            row_sum<TPR, 1>(far, red0, 0);
+            const float mid = far[0] / p.D;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = (k * TPR + lane) * VW;
+#pragma unroll
+                for (int i = 0; i < VW; ++i) {
+                    const float d = END == ROW_FULL || c + i < p.D ? fmaf(v[k][i], 0x1p-80f, -mid) : 0.f;
+                    dev[0] += d;
+                    dev[1] = fmaf(d, d, dev[1]);
+                }
+            }
+            row_sum<TPR, 2>(dev, red1, 0);
+            const float left = dev[0] / p.D, var = dev[1] / p.D - left * left;
+            const float sum = (var < 0.f ? 0.f : var) + p.eps * 0x1p-80f * 0x1p-80f;
+            mean = (mid + left) * 0x1p80f;
+            rstd = sum == 0.f ? 1.f / sqrtf(p.eps) : 0x1p-80f / sqrtf(sum);
+        }
         if (!live) continue;   // whole rows only: no barrier is skipped (TPR > 64 has one row per workgroup, live for all)
         if (lane == 0) {
             if (p.mean) p.mean[row] = mean;
