@@ -21,11 +21,25 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-u
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
-def _stale(out, deps):
-    if not os.path.exists(out):
+def _stale(out, deps, recipe):
+    """out is missing, older than a file it is made of, or was not made (to the end) by this recipe, which lies in <out>.cmd"""
+    try:
+        with open(out + ".cmd") as f:
+            made_by = f.read()
+        t = os.path.getmtime(out)
+    except OSError:
         return True
-    t = os.path.getmtime(out)
-    return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
+    return made_by != recipe or any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
+
+
+def _begin(out):
+    if os.path.exists(out + ".cmd"):
+        os.remove(out + ".cmd")
+
+
+def _done(out, recipe):
+    with open(out + ".cmd", "w") as f:
+        f.write(recipe)
 
 
 def build(force=False, verbose=False):
@@ -41,26 +55,34 @@ def build(force=False, verbose=False):
             continue
         obj = os.path.join(objdir, os.path.splitext(s)[0] + ".o")
         objs.append(obj)
-        if force or _stale(obj, [src] + hdrs):
+        recipe = " ".join([hipcc] + FLAGS + [s])   # (no paths: the tree may be built in one place and used in another)
+        if force or _stale(obj, [src] + hdrs, recipe):
             cmd = [hipcc] + FLAGS + ["-x", "hip", "-c", src, "-o", obj]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            procs.append((s, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+            _begin(obj)
+            procs.append((s, obj, recipe, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
     failed = False
-    for s, p in procs:
+    for s, obj, recipe, p in procs:
         out = p.communicate()[0].decode()
         if p.returncode != 0:
             failed = True
             sys.stderr.write(f"--- {s} ---\n{out}\n")
-        elif verbose and out.strip():
+            continue
+        _done(obj, recipe)
+        if verbose and out.strip():
             print(f"--- {s} ---\n{out}")
     if failed:
         raise RuntimeError("hipcc failed")
-    if force or procs or _stale(LIB, objs):
-        cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
+    link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC"]
+    recipe = " ".join(link + [os.path.basename(o) for o in objs])
+    if force or procs or _stale(LIB, objs, recipe):
+        cmd = link + ["-o", LIB] + objs
         if verbose:
             print(" ".join(cmd), flush=True)
+        _begin(LIB)
         subprocess.check_call(cmd)
+        _done(LIB, recipe)
     return LIB
 
 
