@@ -70,3 +70,12 @@ def test_an_object_of_a_failed_run_is_compiled_again(tree):
         tree()
     (tree.path / "broken").unlink()
     assert tree() == ["lib.so", "two.o"]   # (the failed run left a two.o that is newer than its source)
+
+
+def test_the_build_check_compiles_every_time(monkeypatch):
+    """__graft_entry__.build() answers "does it build": built files that are there do not answer it"""
+    import __graft_entry__ as g
+    seen = []
+    monkeypatch.setattr(b, "build", lambda force=False, verbose=False: seen.append(force) or b.LIB)
+    g.build()
+    assert seen == [True]
