@@ -79,3 +79,40 @@ def test_the_build_check_compiles_every_time(monkeypatch):
     monkeypatch.setattr(b, "build", lambda force=False, verbose=False: seen.append(force) or b.LIB)
     g.build()
     assert seen == [True]
+
+
+def _tool(name):
+    import importlib.util
+    spec = importlib.util.spec_from_file_location(name, os.path.join(ROOT, "tools", name + ".py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    return mod
+
+
+@pytest.mark.parametrize("check", ["hot_loops", "arrival_counter_waits", "mfma_fresh_operand_reads"])
+def test_isa_checks_judge_the_code_that_is_built(check, monkeypatch):
+    """a check of waits and hazards says something of the library only if it compiles the sources with the library's flags"""
+    mod, seen = _tool("isa_loop_check"), []
+
+    class Nothing:
+        stdout = ""
+
+    monkeypatch.setattr(mod.subprocess, "run", lambda cmd, **kw: seen.append(cmd) or Nothing)
+    getattr(mod, check)()
+    assert seen and all(all(f in cmd for f in b.FLAGS) for cmd in seen), seen
+
+
+@pytest.mark.parametrize("script,first", [("build_variant_tu.sh", "act8"), ("build_variant.sh", "pivotcvae_amd/csrc/catalog_bf16.hip")])
+def test_variant_libraries_differ_in_one_source_alone(script, first, tmp_path):
+    """the variant's own unit with the library's flags (and the given one), and every other object of the library beside it"""
+    import subprocess
+    log, cc = tmp_path / "calls", tmp_path / "cc"
+    cc.write_text('#!/bin/sh\necho "$@" >> %s\n' % log)
+    cc.chmod(cc.stat().st_mode | stat.S_IEXEC)
+    subprocess.run(["bash", os.path.join(ROOT, "tools", script), first, str(tmp_path / "v.so"), "-DVARIANT"], check=True, cwd=ROOT,
+                   env=dict(os.environ, HIPCC=str(cc)), stdout=subprocess.DEVNULL)
+    compiled, linked = (line.split() for line in log.read_text().splitlines())
+    assert "-DVARIANT" in compiled and all(f in compiled for f in b.FLAGS)
+    objects = {os.path.basename(o) for o in linked if o.endswith(".o")}
+    own = os.path.splitext(os.path.basename(first))[0] + ".o"
+    assert objects == {os.path.splitext(s)[0] + ".o" for s in b.SOURCES} - {own} | {"v.o"}

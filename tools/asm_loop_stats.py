@@ -1,11 +1,13 @@
 #!/usr/bin/env python3
 """Instruction mix of the hottest loop of one kernel:  asm_loop_stats.py file.hip kernel_substring [--dump]"""
-import re, subprocess, sys
+import os, re, subprocess, sys
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from pivotcvae_amd import build
 from collections import Counter
 src, pat = sys.argv[1], sys.argv[2]
 dump = "--dump" in sys.argv
 asm = "/tmp/_loopstats.s"
-subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only", "-x", "hip", src, "-o", asm],
+subprocess.run(["/opt/rocm/bin/hipcc", *build.FLAGS, "-S", "--cuda-device-only", "-x", "hip", src, "-o", asm],
                stderr=subprocess.DEVNULL, check=True)
 a = open(asm).read()
 starts = [m for m in re.finditer(r"^(_Z\S+):\s*; @", a, re.M)]

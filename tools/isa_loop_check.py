@@ -12,6 +12,9 @@ import subprocess
 import sys
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+if ROOT not in sys.path:
+    sys.path.insert(0, ROOT)
+from pivotcvae_amd import build  # noqa: E402
 FORBIDDEN = ("v_accvgpr_", "v_mov_b", "scratch_", "buffer_store", "v_readlane", "v_writelane")
 
 
@@ -97,12 +100,11 @@ _ASM_CACHE = {}
 
 
 def _asm_of(src, extra=()):
-    """gfx950 ISA of one translation unit (hipcc -S), compiled once per process"""
+    """gfx950 ISA of one translation unit with the library's flags (hipcc -S), compiled once per process"""
     key = (src, tuple(extra))
     if key not in _ASM_CACHE:
-        _ASM_CACHE[key] = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only",
-                                          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",   # as build.FLAGS
-                                          "-x", "hip", *extra, src, "-o", "-"], capture_output=True, text=True, check=True).stdout
+        _ASM_CACHE[key] = subprocess.run(["/opt/rocm/bin/hipcc", *build.FLAGS, "-S", "--cuda-device-only", "-x", "hip", *extra, src, "-o", "-"],
+                                         capture_output=True, text=True, check=True).stdout
     return _ASM_CACHE[key]
 
 
@@ -151,8 +153,7 @@ def arrival_counter_waits(sources=("gemm_f32.hip", "elementwise.hip")):
     bad, seen = [], 0
     for f in sources:
         src = os.path.join(ROOT, "pivotcvae_amd", "csrc", f)
-        asm = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-S", "--cuda-device-only", "-x", "hip",
-                              src, "-o", "-"], capture_output=True, text=True, check=True).stdout
+        asm = _asm_of(src)
         for m in re.finditer(r"^(_Z\S+):\s*; @", asm, re.M):
             body = asm[m.end():asm.find(".Lfunc_end", m.end())].split("\n")
             lines = [l.split(";")[0].strip() for l in body]

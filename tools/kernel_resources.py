@@ -1,19 +1,24 @@
 #!/usr/bin/env python3
 """Compact per-kernel register/LDS/occupancy table for one .hip file (hipcc -Rpass-analysis)."""
+import os
 import re
 import subprocess
 import sys
 
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from pivotcvae_amd import build  # noqa: E402
+
 src = sys.argv[1]
 filt = sys.argv[2] if len(sys.argv) > 2 else ""
-out = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-x", "hip", "-c", src,
-                      "-o", "/dev/null", "-Rpass-analysis=kernel-resource-usage"], capture_output=True, text=True).stderr
+out = subprocess.run(["/opt/rocm/bin/hipcc", *build.FLAGS, "-x", "hip", "-c", src, "-o", "/dev/null", "-Rpass-analysis=kernel-resource-usage"], capture_output=True, text=True).stderr
 cur = None
 rows = []
 for line in out.splitlines():
     m = re.search(r"Function Name: (\S+)", line)
     if m:
-        cur = {"name": subprocess.run(["c++filt", m.group(1)], capture_output=True, text=True).stdout.strip()}
+        cur = {"name": subprocess.run(["c++filt", m.group(1).replace("DF16b", "s").replace("DF16_", "t")], capture_output=True, text=True).stdout.strip()}
+        # (c++filt knows neither __bf16 nor _Float16 in template arguments: they go through it as short and unsigned short)
+        cur["name"] = cur["name"].replace("unsigned short", "_Float16").replace("short", "__bf16")
         rows.append(cur)
         continue
     for key, pat in (("vgpr", r" VGPRs: (\d+)"), ("agpr", r"AGPRs: (\d+)"), ("sgpr", r" SGPRs: (\d+)"),
