@@ -758,8 +758,11 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, checkpoint=None):
     """layer norm over the last dimension (layer_norm_fwd_raw), differentiable; checkpoint = "e4m3": the backward pass reads x from its
-    8-bit form (1.03 bytes per value kept) instead of x itself"""
-    return _LayerNorm.apply(x, weight, bias, float(eps), _check_checkpoint(checkpoint))
+    8-bit form (1.03 bytes per value kept) instead of x itself.  Where no backward pass can follow, nothing is kept"""
+    _check_checkpoint(checkpoint)
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        checkpoint = None
+    return _LayerNorm.apply(x, weight, bias, float(eps), checkpoint)
 
 
 class _KeptStack(torch.autograd.Function):
