@@ -449,9 +449,10 @@ int pcvae_layer_norm_bwd(const void* g, int64_t ldg, int type, int64_t M, int D,
  * Activation checkpoints in 8 bits: what a layer keeps of its input for the backward pass, at 1.03 bytes per value.  No counterpart in
  * the reference (autograd keeps fp32).
  *     Of every row, 32 consecutive columns share one scale byte s (2^(s - 127), s >= 10: the smallest power of two with
- *     max |x| <= 448 * scale over the finite values, |x| held at 1.875 * 2^127); a code is the nearest OCP e4m3 multiple of it, ties to
- *     even; a positive value never becomes zero (it becomes the smallest code: LeakyReLU' reads off the codes exactly); NaN and +-inf
- *     become NaN.  codes [M, ldc], ldc a multiple of 16, >= 32 ceil(D / 32), 16-byte aligned, columns from D on hold code 0;
+ *     max |x| <= 448 * scale over the finite values, |x| held at 1.875 * 2^127, in fp16 rows at 61440: finite values come back finite);
+ *     a code is the nearest OCP e4m3 multiple of it, ties to even; a positive value never becomes zero (it becomes the smallest code:
+ *     LeakyReLU' reads off the codes exactly); NaN and +-inf become NaN.  codes [M, ldc], ldc a multiple of 16, >= 32 ceil(D / 32),
+ *     16-byte aligned, columns from D on hold code 0;
  *     scales [ceil(M / 8)][ceil(D / 32)][8]: the bytes of 8 rows side by side, ldsc bytes per 8 rows (a multiple of 8, >= 8 ceil(D / 32)),
  *     8-byte aligned; the bytes of rows from M on are neither written nor used.
  *     pack       : x -> codes, scales                         unpack : codes, scales -> y (the values, rounded to `type`)

@@ -6,8 +6,8 @@
 // significand bit, makes the division exact - the rounding of the code is the only one - and keeps every value a bf16 as well: byte >= 10
 // keeps the smallest code (2^-9 scale) at 2^-126, a normal number.  Two additions serve the backward pass: a positive value never becomes
 // zero (it becomes the smallest code), so "x > 0" - LeakyReLU's derivative - reads off the code exactly; and NaN / +-inf become the NaN
-// code and stay out of the maximum, so one bad value does not hide its 31 neighbours.  |x| is held at 1.875 * 2^127 (the largest fp32 values
-// would round to 2^128).
+// code and stay out of the maximum, so one bad value does not hide its 31 neighbours.  |x| is held at 1.875 * 2^127, in rows of fp16 at
+// 1.875 * 2^15: the type's largest values would round to 2^128 / 2^16 and come back as infinities.
 #pragma once
 #include "common.h"
 #include <hip/hip_bf16.h>
@@ -24,8 +24,11 @@ template <int BYTES>
 struct __attribute__((packed)) Raw { uint32_t w[BYTES / 4]; };
 
 template <typename T> struct RowType;
+constexpr uint32_t kAct8Cap = 0x7f700000u;      // 1.875 * 2^127
+constexpr uint32_t kAct8CapHalf = 0x47700000u;  // 1.875 * 2^15
 template <> struct RowType<float> {
     static constexpr int VW = 4;
+    static constexpr uint32_t CAP = kAct8Cap;   // (bits of) the largest magnitude an 8-bit row of this type holds
     static __device__ __forceinline__ float one(const float* p) { return *p; }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
     static __device__ __forceinline__ void widen(const Raw<16>& r, float (&v)[4]) {
@@ -43,6 +46,7 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 template <> struct RowType<__bf16> {
     static constexpr int VW = 8;
+    static constexpr uint32_t CAP = kAct8Cap;
     static __device__ __forceinline__ float one(const __bf16* p) {
         return __uint_as_float((uint32_t)*reinterpret_cast<const uint16_t*>(p) << 16);
     }
@@ -64,6 +68,7 @@ template <> struct RowType<__bf16> {
 };
 template <> struct RowType<_Float16> {
     static constexpr int VW = 8;
+    static constexpr uint32_t CAP = kAct8CapHalf;
     static __device__ __forceinline__ float one(const _Float16* p) { return (float)*p; }
     static __device__ __forceinline__ void put(_Float16* p, float v) { *p = (_Float16)v; }
     static __device__ __forceinline__ void widen(const Raw<16>& r, float (&v)[8]) {
@@ -190,7 +195,6 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
 }
 
 // ---- 8-bit blocks -----------------------------------------------------------------------------------------------------------------
-constexpr uint32_t kAct8Cap = 0x7f700000u;   // 1.875 * 2^127
 __device__ __forceinline__ uint32_t act8_byte(uint32_t top) {
     const uint32_t e = (top + 0x1fffffu) >> 23;
     return e > 18u ? e - 8u : 10u;
@@ -199,8 +203,7 @@ __device__ __forceinline__ float act8_inverse(uint32_t byte) { return __uint_as_
 __device__ __forceinline__ float act8_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // four values -> four codes (the lowest byte is the first).  Any values:
-__device__ __forceinline__ uint32_t act8_codes_any(const float* x, float inv) {
-    const float cap = __uint_as_float(kAct8Cap);
+__device__ __forceinline__ uint32_t act8_codes_any(const float* x, float inv, float cap) {
     float v[4];
     uint32_t bad = 0;
 #pragma unroll
@@ -235,10 +238,12 @@ __device__ __forceinline__ B* act8_scale_at(B* scales, int64_t ld, int64_t row, 
     return scales + (row >> 3) * ld + (c / kAct8Block) * 8 + (row & 7);
 }
 
-// a lane's VW values at columns [c, c + VW) of a block it shares with its 32 / VW - 1 neighbours -> codes and (first lane) the scale byte.
+// a lane's VW values of type T at columns [c, c + VW) of a block it shares with its 32 / VW - 1 neighbours -> codes and (first lane) the scale byte.
 // Every lane of the block takes part, whatever its columns (values from D on are zeros); columns from D on get code 0.
-template <int VW>
-__device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, uint8_t* codes, uint8_t* scale) {
+template <typename T>
+__device__ __forceinline__ void act8_store(const float (&v)[RowType<T>::VW], int c, int Dp, uint8_t* codes, uint8_t* scale) {
+    constexpr int VW = RowType<T>::VW;
+    constexpr uint32_t CAP = RowType<T>::CAP;
     // magnitudes as integers: NaN and infinity are the largest.  3.5 vector operations per value unless a lane of the wave holds a bad, a
     // huge or a tiny (zero) value; then the block's maximum is taken again over the finite ones.
     uint32_t top = 0, low = 0xffffffffu;
@@ -249,13 +254,13 @@ __device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, 
         low = a < low ? a : low;
     }
     top = lanes_max<kAct8Block / VW>(top);
-    const bool odd = top > kAct8Cap;   // (uniform over the block's lanes)
+    const bool odd = top > CAP;   // (uniform over the block's lanes)
     if (odd) {
         top = 0;
 #pragma unroll
         for (int i = 0; i < VW; ++i) {
             uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-            a = a >= 0x7f800000u ? 0u : (a < kAct8Cap ? a : kAct8Cap);
+            a = a >= 0x7f800000u ? 0u : (a < CAP ? a : CAP);
             top = a > top ? a : top;
         }
         top = lanes_max<kAct8Block / VW>(top);
@@ -265,7 +270,7 @@ __device__ __forceinline__ void act8_store(const float (&v)[VW], int c, int Dp, 
     uint32_t w[VW / 4];
     if (odd || low < (byte - 9u) << 23) {
 #pragma unroll
-        for (int h = 0; h < VW / 4; ++h) w[h] = act8_codes_any(v + 4 * h, inv);
+        for (int h = 0; h < VW / 4; ++h) w[h] = act8_codes_any(v + 4 * h, inv, __uint_as_float(CAP));
     } else {
 #pragma unroll
         for (int h = 0; h < VW / 4; ++h) w[h] = act8_codes_plain(v + 4 * h, inv);

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(256) void act8_rows_kernel(RowsParams p) {
         float v[VW];
         if constexpr (WHAT == ROWS_PACK) {
             piece_values<T>(xr, static_cast<const T*>(p.x) + r * p.ldx, c, p.D, p.end, true, v);
-            act8_store<VW>(v, c, p.Dp, p.codes + r * p.ldc, act8_scale_at(p.scales, p.lds, r, c));
+            act8_store<T>(v, c, p.Dp, p.codes + r * p.ldc, act8_scale_at(p.scales, p.lds, r, c));
         } else {
             act8_values(qr.w[0], scale, v);
             if constexpr (VW == 8) act8_values(qr.w[1], scale, v + 4);

@@ -156,7 +156,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void layer_norm_fwd_kernel(F
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int c = (k * TPR + lane) * VW;
-            if constexpr (KEEP) act8_store<VW>(v[k], c, p.Dp, p.codes + row * p.ldc, act8_scale_at(p.scales, p.lds, row, c));
+            if constexpr (KEEP) act8_store<T>(v[k], c, p.Dp, p.codes + row * p.ldc, act8_scale_at(p.scales, p.lds, row, c));
             float o[VW];
 #pragma unroll
             for (int i = 0; i < VW; ++i) o[i] = fmaf((v[k][i] - mean) * rstd, w[k][i], b[k][i]);

@@ -189,3 +189,21 @@ def test_codes_and_scales_behind_offsets_over_32_bits():
     _hip.check(L.pcvae_act8_bwd_weight(gz.data_ptr(), N, 0, *far, M, N, D, mean.data_ptr(), rstd.data_ptr(), w.data_ptr(), b.data_ptr(), dW.data_ptr(), D,
                                        dz.data_ptr(), 0, ws.data_ptr(), n, st))
     assert torch.equal(dW, ww[0]) and torch.equal(dz, ww[1])
+
+
+# ---- the largest fp16 values ------------------------------------------------------------------------------------------------------------------
+def test_finite_fp16_rows_come_back_finite():
+    """65504 is nearest to 65536 among its scale's multiples, an infinity in fp16: fp16 rows are held at 61440 (2^-4 of their value off at
+    most, as every code), alone and from the norm's pass; infinities stay NaN"""
+    top = torch.arange(0x7a00, 0x7c00, dtype=torch.int16).view(torch.float16)     # 49152 .. 65504
+    x = torch.cat([top, -top, rand((1024,), 1, torch.float16), torch.full((32,), 65504.0).half()]).view(-1, 32)
+    want = kept64(x.clamp(-61440, 61440))
+    ck = ops().act8_pack(x.to(DEV))
+    got = ck.unpack().cpu()
+    assert got.dtype == torch.float16 and bool(got.isfinite().all()) and torch.equal(got.double(), want)
+    assert bool(((got.double() - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -13).all())   # (ordinary rows: blocks below 8)
+    assert torch.equal(ops().layer_norm_fwd_raw(x.to(DEV), checkpoint="e4m3")[3].codes, ck.codes)
+    assert torch.equal(ops().act8_pack(x.float().to(DEV)).unpack(torch.float32).double().cpu(), kept64(x.float()))   # fp32 rows: as they were
+    x[0, 5] = float("inf")
+    got = ops().act8_pack(x.to(DEV)).unpack().cpu()
+    assert bool(got[0, 5].isnan()) and int(got.isnan().sum()) == 1 and not bool(got.isinf().any())
