@@ -456,11 +456,13 @@ int pcvae_layer_norm_bwd(const void* g, int64_t ldg, int type, int64_t M, int D,
  *     scales [ceil(M / 8)][ceil(D / 32)][8]: the bytes of 8 rows side by side, ldsc bytes per 8 rows (a multiple of 8, >= 8 ceil(D / 32)),
  *     8-byte aligned; the bytes of rows from M on are neither written nor used.
  *     pack       : x -> codes, scales                         unpack : codes, scales -> y (the values, rounded to `type`)
- *     leaky_bwd  : g *= LeakyReLU'(x) in place, x the packed LeakyReLU output
+ *     leaky_bwd  : g *= LeakyReLU'(x) in place, x the packed LeakyReLU output (a NaN code takes the negative side's slope)
  *     bwd_weight : dW[N, K] = sum_m g[m, n] q[m, k],  db[n] = sum_m g[m, n] (NULL: not wanted), q [M, K] the packed values; accumulate:
  *                  added to what is there.  With mean / rstd [M] (and weight / bias [K], NULL: 1 / 0) of a layer norm over q, q is
- *                  replaced by (q - mean) rstd weight + bias.  fp32-exact products (bf16 components of g; the codes are exact in bf16),
- *                  fp32 sums in a fixed order: the same bits every run.  ws: pcvae_act8_bwd_weight_ws_bytes(M, N, K) bytes.
+ *                  replaced by (q - mean) rstd weight + bias.  fp32-exact products (bf16 components of g; the codes are exact in bf16)
+ *                  where |g| (behind a norm |g rstd|) lies in [2^-110, 3.39e38]; smaller ones lose low bits, an infinite or NaN g[m, n]
+ *                  makes row n of dW NaN.  fp32 sums in a fixed order: the same bits every run.  ws:
+ *                  pcvae_act8_bwd_weight_ws_bytes(M, N, K) bytes.
  * ------------------------------------------------------------------------------------------- */
 int pcvae_act8_pack(const void* x, int64_t ldx, int type, int64_t M, int64_t D, uint8_t* codes, int64_t ldc, uint8_t* scales,
                     int64_t ldsc, pcvae_stream_t stream);

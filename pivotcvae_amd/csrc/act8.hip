@@ -5,11 +5,13 @@
 //   weight   dW[N, K] = sum_m g[m, n] q[m, k],  db[n] = sum_m g[m, n]   from the codes of q [M, K]; with q behind a layer norm
 //            (h = (q - mu_m) r_m, the layer's input w_k h + b_k):  dW = w_k (sum_m (g r_m) q - sum_m g r_m mu_m) + b_k db
 //
-// Bounds.  The row kernels: memory (8192 x 5397 fp32 pack 50 us = 4.4 TB/s of codes and values, unpack 35-50 us; a device copy runs at
-// 4.95 TB/s).  The weight gradient: the matrix pipe - 4864 x 1024 over 32768 rows, fp32 g, 850-920 us = 355-384 TFLOP/s of fp32-exact
-// products = 1065-1150 TFLOP/s of bf16 products issued, 0.87-0.94 of what the library's largest bf16 product reaches (1225) - and, for one
-// component (bf16 g), the instructions around its products: 2048 x 2048 over 16384 rows 172 us = 800 TFLOP/s (matrix pipe 0.36 busy, LDS 0.27, vector
-// issue 0.28: two waves per SIMD do not cover each other's waits).  Small ones are launches and latency: 256 x 256 over 8192 rows 24 us.
+// Bounds.  The row kernels: memory (8192 x 5397 fp32 pack 53 us = 4.2 TB/s of codes and values, unpack 35 us, the codes partly cached;
+// LeakyReLU' over 8192 x 256 fp32 7 us, over 32768 x 2048 fp32 102 us; a device copy runs at 4.96 TB/s).  The weight gradient: the matrix pipe -
+// 4864 x 1024 over 32768 rows, fp32 g, 923 us (868 at best) = 354 TFLOP/s of fp32-exact products = 1061 TFLOP/s of bf16 products issued, 0.87
+// of what the library's largest bf16 product reaches (1222); its pipe is 0.52 busy by the counters, 8 registers spill - and, for one
+// component (bf16 g), the instructions around its products: 2048 x 2048 over 16384 rows 178 us = 773 TFLOP/s (matrix pipe 0.35 busy, LDS 0.26, vector
+// issue 0.27: two waves per SIMD do not cover each other's waits); two components (fp16 g) 257 us, behind a norm three whatever g's type: 340-370
+// us.  Small ones are launches and latency: 256 x 256 over 8192 rows 24 us.
 #include "act8.h"
 
 using namespace pcvae;
@@ -113,7 +115,9 @@ int check_plain_rows(const char* who, int type, int64_t M, int64_t D, int64_t ld
 // ---- weight gradient ------------------------------------------------------------------------------------------------------------
 // A product's codes are exact in bf16 (act8.h), so fp32 g needs only its own split: g = c0 + c1 + c2 (three RNE bf16 components whose
 // sum IS the fp32 value), three v_mfma_f32_32x32x16_bf16 per product, fp32 accumulate: fp32 products at a third of the bf16 rate.
-// fp16 g is exact in two components, bf16 g in one; behind a norm the factor g r_m is an fp32 number again (three).
+// fp16 g is exact in two components, bf16 g in one; behind a norm the factor g r_m is an fp32 number again (three).  Exact means |g| (behind
+// a norm |g r_m|) from 2^-110, below which components are too small for a bf16 and vanish one after the other, to 3.39e38, above which the
+// first rounds to an infinity; an infinite g makes its row of dW NaN (its db keeps the infinity).
 //
 // One workgroup: 128 (n) x 64 KT (k) of dW over a range of rows m, four waves of 64 x 32 KT.  Both operands run ALONG the contraction in
 // memory's slow direction, so a chunk of 32 rows is turned on its way to LDS: a wave takes 8 consecutive rows, a lane holds 2 (KT)
@@ -337,8 +341,9 @@ __global__ __launch_bounds__(256, 2) void act8_weight_kernel(DwParams p) {
     };
 
     // The order of a half of the loop, for three components: one product, five vector operations of the next chunk's conversion (what a
-    // product hides: four or five, measured on two waves per SIMD), the operand reads ahead and the stores behind.  4864 x 1024 over 32768
-    // rows 924 -> 911 us, 1024 x 2048 over 16384 rows 220 -> 208 us; with one or two components the compiler's own order is as good.
+    // product hides: four or five, measured on two waves per SIMD), the operand reads ahead and the stores behind.  Kernel and
+    // join, both sides in turn: 4864 x 1024 over 32768 rows 866 -> 847 us, 1024 x 2048 over 16384 rows 191 -> 188 us, behind a norm 213 -> 205
+    // us; with one or two components the compiler's own order is as good.
     auto weave = [&]() {
         if constexpr (NC == 3 && KT == 4) {
             constexpr int PRODUCTS = 4 * NC * KT, READS = KT + 4 * NC - 2, STORES = 2 * NC + KT;
@@ -538,9 +543,12 @@ __global__ __launch_bounds__(256) void act8_weight_empty_kernel(DwParams p) {
 
 // Tile width and ranges of rows.  The wide tile (128 x 256) converts less per product, the narrow one (128 x 128) has two chunks in flight
 // and half the partial tile per range: measured on 8192 rows, us of 128 / 256 columns: 256 x 256 24 / 27, 256 x 1419 43 / 42, 1152 x 256
-// 38 / 37; on 16384 rows 1024 x 2048 245 / 212; 32768 rows 4864 x 1024 1120 / 905.  It is taken from 2048 chunks of 32 rows on, over all tiles.
+// 38 / 37; on 16384 rows 1024 x 2048 245 / 212; 32768 rows 4864 x 1024 1120 / 905.  It is taken from 2048 chunks of 32 rows on, over all tiles -
+// all of these at widths that both tiles pad alike; the rule does not look at padding (K in 257 .. 384 computes 512 columns where the narrow
+// tile would compute 384: 1024 x 300 over 16384 rows 67 us).
 // Ranges: the fewest rounds of 512 resident workgroups, a chunk's time against the partial tiles' traffic (flat: within 5 % over a factor
-// of two in the number of ranges).
+// of two in the number of ranges), 64 at most: one or two tiles over a long batch do not fill the chip (65536 rows: 128 x 257 61 us, 16 x
+// 256 57 us).  A single column (N = 1) takes every chunk the way a range's last one goes: 65536 rows, K = 200 111 us.
 struct DwPlan { int kt, nn, nk, nz; int64_t m_per; };
 DwPlan dw_plan(int64_t M, int64_t N, int64_t K) {
     DwPlan d;

@@ -327,9 +327,9 @@ __device__ __forceinline__ void gemm_tile_dma(const GemmParams& p, const int bx,
                 }
 #else
                 // the split, two values at a time: v_cvt_pk_bf16_f32 rounds a PAIR (RNE) into one register - already the fragment's
-                // layout -, one shift and one mask widen it back, one v_pk_add_f32 takes the (exact) remainders: 4 vector
-                // instructions per pair and level.  Written on explicit 2-vectors: left to itself hipcc packed only every other pair
-                // and split the rest value by value (7 instructions per pair and level; ISA, round 6).  Same roundings, same bits.
+                // layout -, one shift and one mask widen it back, two v_sub_f32 take the (exact) remainders: 5 vector instructions
+                // per pair and level (bf16x6, per chunk: 48 conversions, 64 subtractions, 32 shifts, 32 masks).  Written on explicit
+                // 2-vectors: left to itself hipcc packs only every other pair and converts the rest value by value.  Same bits.
                 unsigned* ph = reinterpret_cast<unsigned*>(&hi);
                 unsigned* pl = reinterpret_cast<unsigned*>(&lo);
                 unsigned* p2 = reinterpret_cast<unsigned*>(&lo2);

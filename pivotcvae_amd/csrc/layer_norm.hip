@@ -13,8 +13,10 @@
 // The backward's column sums: a thread owns columns, so dw and db accumulate in its registers over all rows of its workgroup; the
 // workgroups' partial rows [G, 2, D] are joined in workgroup order by a second kernel (no atomics: the same bits every run).
 //
-// Bound: memory.  Beside a device copy's rate (4.95 TB/s over 2 x 134 MB): forward 32768 x 2048 bf16 56 us = 4.8 TB/s, 16384 x 2048 fp32
-// 51 us = 5.2 TB/s; backward 32768 x 2048 bf16 82 us = 4.9 TB/s, 16384 x 2048 fp32 from its 8-bit form 51 us; one row of 256 1.6 us.
+// Bound: memory.  Beside a device copy's rate (4.96 TB/s over 2 x 2 GiB): forward 32768 x 2048 bf16 56 us = 4.8 TB/s, 16384 x 2048 fp32
+// keeping its 8-bit form 54 us = 5.6 TB/s (inputs partly cached); backward 32768 x 2048 bf16 83 us = 4.9 TB/s, 16384 x 2048 fp32 from its
+// 8-bit form 52 us = 5.9 TB/s; one row of 256 1.8 us.  Past 8192 columns the backward does not fit its registers (plan()): 4096 x 16384
+// fp32 229 us = 3.5 TB/s, bf16 99 us = 4.1 TB/s, from the 8-bit form 231 and 155 us; the forward holds 5.6 and 5.0 TB/s there.
 // A piece is one 16-byte load whatever the width and alignment of the rows (value-by-value tails behind branches: 104 / 129 us instead
 // of 56 / 82 on the bf16 case), and the next row's loads are in flight over the current row's sums.
 #include "act8.h"
@@ -322,7 +324,8 @@ __global__ __launch_bounds__(1024) void column_join_kernel(const float* part, in
 
 // threads per row and 16-byte pieces per thread for a width: one piece each up to a wave, then more pieces per lane of a wave (no barrier)
 // as far as the registers of the backward go - it holds w, dw, db in fp32 per column: 4 pieces of fp32, 2 of the half types -, then 256
-// threads, then 1024
+// threads, then 1024.  The last rung (8193 .. 16384 columns) has as many pieces in 1024 threads, where a thread has 128 registers: the
+// backward spills 10 to 58 of them there (28 to 212 bytes of scratch per lane), the forward none.
 struct Plan { int tpr, nv, end; };
 Plan plan(int D, int vw) {
     const int pieces = (int)cdiv(D, vw);

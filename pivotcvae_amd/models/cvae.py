@@ -94,8 +94,11 @@ class BaseCVAE(nn.Module):
 
     def set_activation_checkpoint(self, name):
         """what a train step keeps of the MLP stacks' activations for its backward pass: None (fp32, the default) or "e4m3" (8 bits: a
-        power-of-two scale per 32 columns, 1.03 bytes per value).  The forward pass and the loss are unchanged; weight gradients (and
-        the norms' gradients) are those at activations rounded to 2^-4 relative, LeakyReLU' stays exact"""
+        power-of-two scale per 32 columns, 1.03 bytes per value).  The forward pass and the loss are unchanged, LeakyReLU' stays exact.
+        Without norms weight gradients are those at activations rounded to 2^-4 relative, and bias and input gradients are unchanged.
+        With ``layer_norm=True`` a norm's backward takes its rows from the 8 bits too: the norms' gradients and every gradient in front
+        of a norm (earlier layers' biases, the stack's input, through z the encoder's and the prior's) are those at rounded rows.
+        What it buys is memory, not time: the stacks run one after another instead of in the fused launches"""
         if name not in ops.ACTIVATION_CHECKPOINTS:
             raise ValueError(f"activation checkpoint {name!r}: one of {ops.ACTIVATION_CHECKPOINTS}")
         self.activation_checkpoint = name

@@ -650,7 +650,8 @@ def act8_leaky_bwd_(g, ck):
 
 def act8_bwd_weight_raw(gy, ck, dW=None, db=None, norm=None):
     """the weight gradient of a linear layer whose input was kept in 8 bits: dW[N, K] = gy^T q, db[N] = column sums of gy
-    (gy [..., N] fp32 / bf16 / fp16, products and sums fp32) -> (dW, db).  Given buffers are accumulated into; None: new ones.
+    (gy [..., N] fp32 / bf16 / fp16, products and sums fp32; a gradient that is not finite makes its row of dW NaN) -> (dW, db).  Given
+    buffers are accumulated into; None: new ones.
     norm = (mean, rstd, weight, bias): the layer's input was layer_norm(q) with those statistics (weight / bias may be None)."""
     mean, rstd, w, b = norm if norm is not None else (None,) * 4
     dev = _one_device(gy, ck.codes, ck.scales, dW, db, mean, rstd, w, b)
