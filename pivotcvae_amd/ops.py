@@ -245,10 +245,11 @@ def linear_bwd_weight_raw(gy, x, dW, db):
 class GemmGroup:
     """Independent layer GEMMs collected into ONE launch (pcvae_linear_group): a layer's weight- and input-gradient, the same
     layer of two stacks that do not feed each other.  The methods mirror linear_fwd_raw / linear_bwd_input_raw /
-    linear_bwd_weight_raw; nothing runs before launch()."""
+    linear_bwd_weight_raw; nothing runs before launch() - unless two problems write one buffer (layers that share a parameter and so
+    its gradient, which is read, added to and written): the first then runs in a launch of its own, in front."""
 
     def __init__(self):
-        self.descs, self.keep, self.flops = [], [], 0.0
+        self.descs, self.keep, self.out, self.flops = [], [], set(), 0.0
         self.mode = _MLP_MODE
 
     def _add(self, kind, act, a, b, c, aux, aux_out, M, N, K):
@@ -258,6 +259,10 @@ class GemmGroup:
         for x in (a, b, c, aux, aux_out):
             if x is not None and x.dtype != F32:
                 raise TypeError(f"expected {F32}, got {x.dtype}")
+        out = {t.data_ptr() for t in (c, aux_out) if t is not None and t.numel()}
+        if self.out & out:
+            self.launch()
+        self.out |= out
         self.descs.append(d)
         self.keep += [a, b, c, aux, aux_out]
         self.flops += 2.0 * M * N * K
@@ -302,7 +307,7 @@ class GemmGroup:
             nbytes = lib().pcvae_linear_group_ws_bytes(arr, len(part))
             ws = _workspace(self.keep[0].device, nbytes, tag="gemm", zero=True) if nbytes else None
             _timed_gemm(flops, lambda: check(lib().pcvae_linear_group(arr, len(part), ptr(ws), nbytes, stream()), "linear_group"))
-        self.descs, self.keep = [], []
+        self.descs, self.keep, self.out = [], [], set()
 
 
 def leaky_bwd_(g, y):

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.gpu_util import DEV
-from tests.norm_act8_ref import SLOPE, TYPES, Norm64, inside, kept64, weight_grad
+from tests.norm_act8_ref import SLOPE, TYPES, U, Norm64, inside, kept64, weight_grad
 from tests.test_hip_norm_act8 import EPS, ops, params, rand
 
 pytestmark = pytest.mark.gpu
@@ -207,3 +207,30 @@ def test_finite_fp16_rows_come_back_finite():
     x[0, 5] = float("inf")
     got = ops().act8_pack(x.to(DEV)).unpack().cpu()
     assert bool(got[0, 5].isnan()) and int(got.isnan().sum()) == 1 and not bool(got.isinf().any())
+
+
+# ---- shared parameters ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("normed,checkpoint", [(False, None), (True, None), (False, "e4m3"), (True, "e4m3")])
+def test_tied_layers_accumulate_into_their_one_gradient(normed, checkpoint):
+    """three layers (and two norms) that are the same parameters, gradients accumulated in place: the sum of what each layer gives on its
+    own.  Per layer and norm one fp32 addition to what is there (zero, exactly, at first): three layers agree to 2 u of the parts'
+    magnitudes per addition, two norms to 2 u in all"""
+    W, M = 192, 3000
+    w = (rand((W, W), 1, leaky=False) / W ** 0.5).to(DEV)
+    x, t = rand((M, W), 3, leaky=False).to(DEV), rand((M, W), 4, leaky=False).to(DEV)
+    grads = []
+    for tied in (True, False):
+        layers = [(w.clone().requires_grad_(), torch.zeros(W, device=DEV).requires_grad_()) for _ in range(1 if tied else 3)]
+        norms = [tuple(p.to(DEV).requires_grad_() for p in params(W, 5)) for _ in range(1 if tied else 2)] if normed else None
+        for p in [q for pair in layers + (norms or []) for q in pair]:
+            p.grad = torch.zeros_like(p)
+        each = 3 // len(layers)
+        (ops().mlp(x, layers * each, True, norms=norms and norms * (2 // len(norms)), checkpoint=checkpoint) * t).sum().backward()
+        grads.append([[p.grad for p in pair] for pair in layers + (norms or [])])
+    tied, single = grads
+    for k in range(2):
+        parts = [single[i][k].double() for i in range(3)]
+        assert bool(((tied[0][k].double() - sum(parts)).abs() <= 4 * U * sum(p.abs() for p in parts)).all())
+        if normed:
+            parts = [single[3 + i][k].double() for i in range(2)]
+            assert bool(((tied[1][k].double() - sum(parts)).abs() <= 2 * U * sum(p.abs() for p in parts)).all())
