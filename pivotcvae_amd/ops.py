@@ -316,6 +316,15 @@ def leaky_bwd_(g, y):
     return g
 
 
+def _held_grad(p):
+    """the gradient buffer a leaf parameter holds, to accumulate into in place, or None.  Asked in the backward pass: between the passes an
+    optimizer's zero_grad() may have let go of the buffer that was there (or autograd have attached one)"""
+    if not (p.is_leaf and p.requires_grad):
+        return None
+    g = p.grad
+    return g if g is not None and g.is_cuda and g.shape == p.shape and g.is_contiguous() else None
+
+
 class _MLP(torch.autograd.Function):
     """A stack of Linear(+LeakyReLU) layers as one autograd node.
 
@@ -345,9 +354,6 @@ class _MLP(torch.autograd.Function):
             acts.append(h)
         ctx.last_linear = last_linear
         ctx.n = n
-        # gradient buffers to accumulate into directly (leaf parameters with a pre-attached, same-shape .grad)
-        ctx.direct = [p.grad if (p.is_leaf and p.requires_grad and p.grad is not None and p.grad.is_cuda
-                                 and p.grad.shape == p.shape and p.grad.is_contiguous()) else None for p in params]
         ctx.save_for_backward(*acts, *params)
         return h
 
@@ -369,7 +375,7 @@ class _MLP(torch.autograd.Function):
         for i in range(n - 1, -1, -1):
             W, b = params[2 * i], params[2 * i + 1]
             if ctx.needs_input_grad[2 + 2 * i] or ctx.needs_input_grad[3 + 2 * i]:
-                dW, db = ctx.direct[2 * i], ctx.direct[2 * i + 1]
+                dW, db = _held_grad(W), _held_grad(b)
                 if dW is None or db is None:   # else: accumulated in place, nothing to hand to autograd
                     dW, db = torch.zeros_like(W), torch.zeros_like(b)
                     grads[2 * i], grads[2 * i + 1] = dW, db
@@ -424,8 +430,6 @@ class _MLPHeads(torch.autograd.Function):
         ya = linear_fwd_raw(h, Wa, ba, ACT_NONE)
         yb = linear_fwd_raw(h, Wb, bb, ACT_NONE)
         ctx.n = n_trunk
-        ctx.direct = [p.grad if (p.is_leaf and p.requires_grad and p.grad is not None and p.grad.is_cuda
-                                 and p.grad.shape == p.shape and p.grad.is_contiguous()) else None for p in params]
         ctx.save_for_backward(*acts, *params)
         return ya, yb
 
@@ -445,7 +449,7 @@ class _MLPHeads(torch.autograd.Function):
         def weight_grad(grp, k, g, a):   # parameter pair k (weight 2k, bias 2k + 1) from output gradient g and layer input a
             if not (ctx.needs_input_grad[2 + 2 * k] or ctx.needs_input_grad[3 + 2 * k]):
                 return
-            dW, db = ctx.direct[2 * k], ctx.direct[2 * k + 1]
+            dW, db = _held_grad(params[2 * k]), _held_grad(params[2 * k + 1])
             if dW is None or db is None:   # else: accumulated in place, nothing to hand to autograd
                 dW, db = torch.zeros_like(params[2 * k]), torch.zeros_like(params[2 * k + 1])
                 grads[2 * k], grads[2 * k + 1] = dW, db
@@ -812,8 +816,6 @@ class _KeptStack(torch.autograd.Function):
             outs = [linear_fwd_raw(h, *layers[n + j], ACT_NONE) for j in range(heads)] or [h]
         ctx.spec, ctx.hidden, ctx.inner = spec, hidden, inner
         if train:
-            ctx.direct = [p.grad if (p.is_leaf and p.requires_grad and p.grad is not None and p.grad.is_cuda
-                                     and p.grad.shape == p.shape and p.grad.is_contiguous()) else None for p in params]
             flat, ctx.layout = [], []
             for pair in keep:
                 place = []
@@ -866,7 +868,7 @@ class _KeptStack(torch.autograd.Function):
         dwg = GemmGroup()
 
         def buffers(k):   # (dW, db) of parameter pair k: its .grad where it owns one (accumulated in place), else new zeros
-            dW, db = ctx.direct[2 * k], ctx.direct[2 * k + 1]
+            dW, db = _held_grad(params[2 * k]), _held_grad(params[2 * k + 1])
             if dW is None or db is None:
                 dW, db = torch.zeros_like(params[2 * k]), torch.zeros_like(params[2 * k + 1])
                 grads[2 * k], grads[2 * k + 1] = dW, db
@@ -1020,6 +1022,13 @@ class _StacksPacked(torch.autograd.Function):
             return _StacksPacked._forward_impl(ctx, spec, *tensors)
 
     @staticmethod
+    def _flat_grads(params):   # views of the flat gradient buffer: accumulated into in place
+        direct = [[q.grad for q in P] for P in params]
+        if any(g is None for D in direct for g in D):
+            raise RuntimeError("mlp_heads_packed needs gradient buffers attached to every parameter (FlatAdam)")
+        return direct
+
+    @staticmethod
     def _forward_impl(ctx, spec, *tensors):
         S = len(spec)
         require_device(*tensors)
@@ -1041,9 +1050,7 @@ class _StacksPacked(torch.autograd.Function):
                     ys[s] = grp.fwd(acts[s][-1], _cat2(Wa, Wb), _cat2(ba, bb), ACT_NONE)
             grp.launch()
         ctx.spec = spec
-        ctx.direct = [[q.grad for q in P] for P in params]   # views of the flat gradient buffer: accumulated into in place
-        if any(g is None for D in ctx.direct for g in D):
-            raise RuntimeError("mlp_heads_packed needs gradient buffers attached to every parameter (FlatAdam)")
+        _StacksPacked._flat_grads(params)
         ctx.save_for_backward(*[a for A in acts for a in A], *[q for P in params for q in P])
         return tuple(ys)
 
@@ -1065,13 +1072,14 @@ class _StacksPacked(torch.autograd.Function):
         for n in spec:
             params.append(saved[pos:pos + 2 * n + 4])
             pos += 2 * n + 4
+        direct = _StacksPacked._flat_grads(params)
         g = [_c2d(x) for x in gs]
         dwg = GemmGroup()   # the weight gradients of every layer of every stack: off the dependency chain, ONE grouped launch (six
         #                     problems per launch) behind the input-gradient chain - the reductions of their batch splits overlap
         for lvl in range(max(spec) + 1):   # level 0 = the heads, level j = trunk layer n - j
             grp = GemmGroup()
             for s, n in enumerate(spec):
-                P, D, need_x = params[s], ctx.direct[s], ctx.needs_input_grad[1 + s]
+                P, D, need_x = params[s], direct[s], ctx.needs_input_grad[1 + s]
                 if lvl == 0:
                     Wa, ba, Wb, bb = P[2 * n:2 * n + 4]
                     dWa, dba, dWb, dbb = D[2 * n:2 * n + 4]
@@ -1180,8 +1188,6 @@ class _MLPInto(torch.autograd.Function):
         width = params[2 * n - 2].shape[0]
         linear_fwd_raw(h, params[2 * n - 2], params[2 * n - 1], ACT_NONE, out=out_buf[:, col0:col0 + width])
         ctx.n, ctx.col0, ctx.width, ctx.grad_cols = n, col0, width, grad_cols
-        ctx.direct = [p.grad if (p.is_leaf and p.requires_grad and p.grad is not None and p.grad.is_cuda
-                                 and p.grad.shape == p.shape and p.grad.is_contiguous()) else None for p in params]
         ctx.save_for_backward(*acts, *params)
         ctx.mark_dirty(out_buf)
         return out_buf
@@ -1202,7 +1208,7 @@ class _MLPInto(torch.autograd.Function):
         for i in range(n - 1, -1, -1):
             W, b = params[2 * i], params[2 * i + 1]
             if ctx.needs_input_grad[4 + 2 * i] or ctx.needs_input_grad[5 + 2 * i]:
-                dW, db = ctx.direct[2 * i], ctx.direct[2 * i + 1]
+                dW, db = _held_grad(W), _held_grad(b)
                 if dW is None or db is None:
                     dW, db = torch.zeros_like(W), torch.zeros_like(b)
                     grads[2 * i], grads[2 * i + 1] = dW, db

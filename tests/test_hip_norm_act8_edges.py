@@ -234,3 +234,37 @@ def test_tied_layers_accumulate_into_their_one_gradient(normed, checkpoint):
         if normed:
             parts = [single[3 + i][k].double() for i in range(2)]
             assert bool(((tied[1][k].double() - sum(parts)).abs() <= 2 * U * sum(p.abs() for p in parts)).all())
+
+
+# ---- gradients cleared between the passes -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("how", ["to none", "to zero", "replaced"])
+@pytest.mark.parametrize("stack", ["mlp", "mlp normed", "mlp kept", "mlp both", "heads", "heads both", "into"])
+def test_gradients_cleared_after_the_forward_pass_arrive_all_the_same(stack, how):
+    """output = f(x); optimizer.zero_grad(); output.backward(): the gradient goes to where the parameter holds it by then"""
+    o, W, M = ops(), 48, 70
+    layers = [((rand((W, W), i, leaky=False) / W ** 0.5).to(DEV).requires_grad_(), torch.zeros(W, device=DEV).requires_grad_()) for i in range(4)]
+    norms = [tuple(p.to(DEV).requires_grad_() for p in params(W, 5 + i)) for i in range(2)]
+    x, t = rand((M, W), 3, leaky=False).to(DEV), rand((M, W), 4, leaky=False).to(DEV)
+    kw = dict(norms=norms if stack.endswith(("normed", "both")) else None, checkpoint="e4m3" if stack.endswith(("kept", "both")) else None)
+    if stack.startswith("mlp"):
+        f, used = lambda: o.mlp(x, layers[:3], True, **kw), layers[:3]
+    elif stack.startswith("heads"):
+        f, used = lambda: sum(o.mlp_heads(x, layers[:2], layers[2], layers[3], **kw)), layers
+    else:
+        f, used = lambda: o.mlp_into(x, layers[:2], torch.zeros(M, W + 8, device=DEV), 8)[:, 8:], layers[:2]
+    leaves = [p for pair in used + (norms if kw["norms"] else []) for p in pair]
+    (f() * t).sum().backward()
+    want = [p.grad.clone() for p in leaves]      # into parameters that held no gradient
+    assert all(bool(g.any()) for g in want)
+    out = (f() * t).sum()                        # ... and now they do
+    old = [p.grad for p in leaves]
+    for p in leaves:
+        if how == "to zero":
+            p.grad.zero_()
+        else:
+            p.grad = None if how == "to none" else torch.zeros_like(p)
+    before = [g.clone() for g in old]
+    out.backward()
+    assert all(p.grad is not None and torch.equal(p.grad, g) for p, g in zip(leaves, want))
+    assert all((p.grad is g) == (how == "to zero") for p, g in zip(leaves, old))
+    assert how == "to zero" or all(torch.equal(g, b) for g, b in zip(old, before))       # buffers let go of are left alone
