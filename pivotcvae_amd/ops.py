@@ -316,6 +316,19 @@ def leaky_bwd_(g, y):
     return g
 
 
+def _flat_layers(layers):
+    """[W, b, W, b, ...] of (weight [out, in], bias [out]) pairs.  The GEMM kernels take a weight by its row stride and as many values of a bias as
+    the weight has rows, as they lie: other column strides would be misread, a shorter bias read past its end"""
+    flat = []
+    for W, b in layers:
+        if W.dim() != 2 or (b is not None and (b.dim() != 1 or b.shape[0] < W.shape[0])):
+            raise RuntimeError(f"layer: weight [out, in] and bias [out] expected, got shapes {tuple(W.shape)} and {None if b is None else tuple(b.shape)}")
+        if (W.shape[1] > 1 and W.stride(1) != 1) or (b is not None and b.shape[0] > 1 and b.stride(0) != 1):
+            raise ValueError("layer: a weight has contiguous rows, a bias is contiguous")
+        flat += [W, b]
+    return flat
+
+
 def _held_grad(p):
     """the gradient buffer a leaf parameter holds, to accumulate into in place, or None.  Asked in the backward pass: between the passes an
     optimizer's zero_grad() may have let go of the buffer that was there (or autograd have attached one)"""
@@ -483,10 +496,7 @@ def mlp_heads(x, trunk, head_a, head_b, norms=None, checkpoint=None, norm_eps=1e
     checkpoint = "e4m3": what the backward pass reads of the activations is kept in 8 bits (_KeptStack)"""
     if norms is not None or checkpoint is not None:
         return _kept_stack(x, trunk, [head_a, head_b], False, norms, checkpoint, norm_eps)
-    flat = []
-    for W, b in list(trunk) + [head_a, head_b]:
-        flat += [W, b]
-    return _MLPHeads.apply(x, len(trunk), *flat)
+    return _MLPHeads.apply(x, len(trunk), *_flat_layers(list(trunk) + [head_a, head_b]))
 
 
 # --------------------------------------------------------------- layer norm, activation checkpoints in 8 bits (csrc/layer_norm.hip, act8.hip)
@@ -933,9 +943,7 @@ def _kept_stack(x, layers, heads, last_linear, norms, checkpoint, eps):
     inner = len(layers) if heads else len(layers) - 1
     if norms is not None and len(norms) != inner:
         raise RuntimeError(f"{len(norms)} norms for {inner} hidden activations")
-    flat = []
-    for pair in list(layers) + list(heads) + list(norms or []):
-        flat += list(pair)
+    flat = _flat_layers(list(layers) + list(heads)) + [t for pair in norms or [] for t in pair]
     for w, b in norms or []:
         if w is None or b is None:
             raise ValueError("a stack's norms have a weight and a bias each")
@@ -1097,10 +1105,7 @@ class _StacksPacked(torch.autograd.Function):
 
 
 def _stack_args(x, trunk, head_a, head_b):
-    flat = []
-    for W, b in list(trunk) + [head_a, head_b]:
-        flat += [W, b]
-    return x, flat
+    return x, _flat_layers(list(trunk) + [head_a, head_b])
 
 
 def mlp_heads_packed(x, trunk, head_a, head_b):
@@ -1235,10 +1240,7 @@ def mlp_into(x, layers, out_buf, col0, grad_cols=None):
         # the columns behind grad_cols of the returned input gradient are UNWRITTEN memory; only latent_packed (which reads the
         # first Z columns and nothing else) may be the producer of x
         raise RuntimeError("mlp_into(grad_cols=...): x must come straight from ops.latent_packed")
-    flat = []
-    for W, b in layers:
-        flat += [W, b]
-    return _MLPInto.apply(x, out_buf, int(col0), None if grad_cols is None else int(grad_cols), *flat)
+    return _MLPInto.apply(x, out_buf, int(col0), None if grad_cols is None else int(grad_cols), *_flat_layers(layers))
 
 
 def mlp(x, layers, last_linear, norms=None, checkpoint=None, norm_eps=1e-5):
@@ -1246,10 +1248,7 @@ def mlp(x, layers, last_linear, norms=None, checkpoint=None, norm_eps=1e-5):
     activation; checkpoint = "e4m3": what the backward pass reads of the activations is kept in 8 bits (_KeptStack)"""
     if norms is not None or checkpoint is not None:
         return _kept_stack(x, layers, [], last_linear, norms, checkpoint, norm_eps)
-    flat = []
-    for W, b in layers:
-        flat += [W, b]
-    return _MLP.apply(x, last_linear, *flat)
+    return _MLP.apply(x, last_linear, *_flat_layers(layers))
 
 
 class _DenseScores(torch.autograd.Function):
@@ -2212,7 +2211,4 @@ class _MLPRelu(torch.autograd.Function):
 
 
 def mlp_relu(x, layers):
-    flat = []
-    for W, b in layers:
-        flat += [W, b]
-    return _MLPRelu.apply(x, *flat)
+    return _MLPRelu.apply(x, *_flat_layers(layers))

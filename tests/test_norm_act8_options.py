@@ -60,3 +60,22 @@ def test_one_launch_never_accumulates_twice_into_a_buffer(monkeypatch):
     got = [[(c, d) for c, d in part] for part in launches]
     at = lambda k, j: (W[k].data_ptr(), b[j].data_ptr())   # noqa: E731
     assert got == [[at(0, 0), at(1, 1)], [at(0, 0), at(2, 1)], [at(2, 2)]]
+
+
+@pytest.mark.parametrize("call", ["mlp", "mlp normed", "mlp kept", "heads", "heads kept", "relu", "into"])
+@pytest.mark.parametrize("W,b,err,say", [(torch.zeros(8, 16)[:, ::2], torch.zeros(8), ValueError, "contiguous rows"), (torch.zeros(8, 8).t(), torch.zeros(8), ValueError, "contiguous rows"),
+                                         (torch.zeros(8, 8), torch.zeros(16)[::2], ValueError, "contiguous"), (torch.zeros(8, 8), torch.zeros(1).expand(8), ValueError, "contiguous"),
+                                         (torch.zeros(8, 8), torch.zeros(7), RuntimeError, "shape"), (torch.zeros(8, 8), torch.zeros(8, 1), RuntimeError, "shape"),
+                                         (torch.zeros(8), torch.zeros(8), RuntimeError, "shape")])
+def test_stacks_refuse_layers_that_the_kernels_would_misread(call, W, b, err, say):
+    """the kernels read weights by rows of unit column stride and one bias per row: anything else is refused before a launch"""
+    x, ok = torch.zeros(4, 8), (torch.zeros(8, 8), torch.zeros(8))
+    norm = [(torch.ones(8), torch.zeros(8))]
+    with pytest.raises(err, match=say):
+        {"mlp": lambda: ops.mlp(x, [ok, (W, b)], True),
+         "mlp normed": lambda: ops.mlp(x, [(W, b), ok], True, norms=norm),
+         "mlp kept": lambda: ops.mlp(x, [ok, (W, b)], True, checkpoint="e4m3"),
+         "heads": lambda: ops.mlp_heads(x, [ok], ok, (W, b)),
+         "heads kept": lambda: ops.mlp_heads(x, [(W, b)], ok, ok, checkpoint="e4m3"),
+         "relu": lambda: ops.mlp_relu(x, [ok, (W, b)]),
+         "into": lambda: ops.mlp_into(x, [(W, b)], torch.zeros(4, 16), 8)}[call]()
