@@ -90,7 +90,7 @@ def _tool(name):
 
 
 @pytest.mark.parametrize("check", ["hot_loops", "arrival_counter_waits", "mfma_fresh_operand_reads"])
-def test_isa_checks_judge_the_code_that_is_built(check, monkeypatch):
+def test_isa_checks_compile_what_is_built(check, monkeypatch):
     """a check of waits and hazards says something of the library only if it compiles the sources with the library's flags"""
     mod, seen = _tool("isa_loop_check"), []
 
